@@ -48,6 +48,13 @@ extern "C" {
 #define B200_ACT_RELU 1
 #define B200_ACT_LEAKY_RELU 2
 
+/* Element types of the serving operators. B200_E4M3: 8 bits, 4 of exponent,
+ * 3 of mantissa, largest value 448. */
+#define B200_F32 0
+#define B200_BF16 1
+#define B200_F16 2
+#define B200_E4M3 3
+
 #define B200_REDUCE_SUM 0  /* acc + x, the tensor_sum body */
 #define B200_REDUCE_PROD 1 /* acc * x */
 #define B200_REDUCE_MAX 2  /* x > acc ? x : acc, the tensor_max body */
@@ -323,6 +330,75 @@ int b200_debug_schedule(int kind, int64_t M, int64_t N, int64_t K, int64_t* out)
  * full PCIe speed; the Python frontend returns its arrays in them. */
 int b200_host_alloc(void** ptr, int64_t bytes);
 int b200_host_free(void* ptr);
+
+/* ----------------------------------------------------- serving a dense network
+ * The operators around the dense layers of a network that is served token by
+ * token: norm, 4-bit dense layer, token log probabilities. Device pointers,
+ * asynchronous on `stream`, no scratch memory: they may be captured into
+ * graphs, and calls on several streams do not share anything. Buffers start
+ * on a multiple of their element size; outputs must not overlap inputs except
+ * where stated. No counterpart in the reference. */
+
+/* Root-mean-square norm of the rows of X[M,N]:
+ *   h = X + R;  y = h / sqrt(mean(h^2) + eps) * w
+ * X, R (or NULL) and H (or NULL: not stored) are of type `dtype`; w[N] (or
+ * NULL: 1) is of that type or f32. H may be X or R itself (same address and
+ * pitch). y is computed in f32 from the f32 sum and rounded once into Y:
+ * of X's type (y_dtype == dtype, scales NULL), or e4m3 codes
+ * (y_dtype B200_E4M3) with scales: the value is code * scale, and
+ * scale = max|y| / 448 over the row (group 0: scales[m * ld_scales]) or over
+ * each `group` (32, 64 or 128) columns (scales[m * ld_scales + n / group];
+ * the last group may be shorter). Where all of y is zero the scale is 1. A
+ * row of X that holds an infinity or NaN gives what the formula gives. */
+int b200_rms_norm(const void* X, int64_t ldx, const void* R, int64_t ldr, int dtype, const void* w,
+                  int w_dtype, float eps, void* H, int64_t ldh, void* Y, int64_t ldy, int y_dtype,
+                  float* scales, int64_t ld_scales, int group, int64_t M, int64_t N, void* stream);
+
+/* 4-bit weights. W[k,n] = scales[k / group, n] * (codes[k,n] - zeros[k / group, n])
+ * with codes and zeros in 0..15 (8 without zeros), one code or zero a byte,
+ * and group 32 or a multiple of 64 (the last group of K may be shorter).
+ * b200_w4_quantize makes codes and scales of f32 weights:
+ * scale = max|w| / 7 over the group, rounded to the scales' type (s_dtype:
+ * f32, bf16 or f16), code = round(w / scale) + 8.
+ * b200_w4_pack lays codes, scales and zeros (or NULL) out as b200_dense_w4
+ * reads them, into b200_w4_bytes(...) bytes at a 16-byte aligned address;
+ * b200_w4_dequantize gives the f32 matrix of packed weights, for example for
+ * b200_dense_f32 on many rows. */
+int64_t b200_w4_bytes(int64_t K, int64_t N, int group, int s_dtype, int has_zeros);
+int b200_w4_quantize(const float* W, int64_t ldw, int64_t K, int64_t N, int group, uint8_t* codes,
+                     int64_t ldc, void* scales, int64_t lds, int s_dtype, void* stream);
+int b200_w4_pack(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds, int s_dtype,
+                 const uint8_t* zeros, int64_t ldz, int64_t K, int64_t N, int group, void* packed,
+                 void* stream);
+int b200_w4_dequantize(const void* packed, int s_dtype, int has_zeros, int64_t K, int64_t N,
+                       int group, float* W, int64_t ldw, void* stream);
+
+/* Y = act(X @ W + b) with W packed by b200_w4_pack, for few rows: X[M,K] of
+ * f32, bf16, f16 or e4m3, Y[M,N] of f32, bf16 or f16, b[N] (or NULL) of f32,
+ * bf16 or f16. An e4m3 X may have x_scales: one for each row (x_group 0,
+ * x_scales[m * ld_x_scales]) or for each x_group (32, 64 or 128) columns, as
+ * b200_rms_norm writes them. Products are exact and sums run in f32 (an f32 X
+ * keeps all its bits); Y is rounded once. The weights are read once for each
+ * 64 rows (f32: 21 rows), so many rows are better served by
+ * b200_w4_dequantize and b200_dense_f32. */
+int b200_dense_w4(const void* X, int64_t ldx, int x_dtype, const float* x_scales,
+                  int64_t ld_x_scales, int x_group, const void* packed, int s_dtype, int has_zeros,
+                  int group, const void* b, int b_dtype, void* Y, int64_t ldy, int y_dtype,
+                  int64_t M, int64_t N, int64_t K, int act, float alpha, void* stream);
+
+/* Over rows of logits [T,V] (f32, bf16 or f16) and p = softmax(row):
+ *   logprobs[t] = log p[tokens[t]]        (tokens and logprobs, or both NULL);
+ *                 0 for a negative token (a padded row), NaN for one >= V
+ *   entropy[t]  = -sum p log p            (or NULL)
+ *   top_logprobs[t * top + i], top_tokens[t * top + i]: the i-th most probable
+ *                 token, the lowest index first among equals (top <= 32, V)
+ * Logits of -inf are masked tokens. A row of nothing else has no
+ * distribution: its log probabilities are -inf, its entropy 0. In a row with
+ * a NaN or +inf logit log probabilities and entropy are NaN; tokens are still
+ * ordered by their logits, NaN last with -inf. */
+int b200_token_logprobs(const void* logits, int64_t ld, int dtype, int64_t T, int64_t V,
+                        const int32_t* tokens, float* logprobs, float* entropy, int top,
+                        float* top_logprobs, int32_t* top_tokens, void* stream);
 
 /* --------------------------------------------------- host-pointer entry points */
 

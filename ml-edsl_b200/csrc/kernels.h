@@ -18,6 +18,8 @@ enum Status : int {
 };
 
 enum Act : int { kActNone = 0, kActRelu = 1, kActLeakyRelu = 2 };
+// Element types of the serving operators (B200_F32 and so on).
+enum Dtype : int { kF32 = 0, kBF16 = 1, kF16 = 2, kE4M3 = 3 };
 enum RedOp : int { kRedSum = 0, kRedProd = 1, kRedMax = 2, kRedMin = 3 };
 
 // Number of kernels this library has launched (process-wide).
@@ -161,6 +163,74 @@ int bias_add_i32(const int32_t* X, int64_t ldx, const int32_t* b, int32_t* Y, in
                  int64_t M, int64_t N, cudaStream_t stream);
 int fill_bias_act_f32(const float* b, float* Y, int64_t ldy, int64_t M, int64_t N, int act,
                       float alpha, cudaStream_t stream);
+
+// ---- norm of rows with residual and 8-bit output (rms_norm.cu). X, R, H
+// (and Y without scales) are of one type; w is of that type, or f32 (w_f32).
+// With scales, Y holds e4m3 codes; group 0 = one scale a row.
+struct RmsNormArgs {
+  const void* X;
+  const void* R;  // or null
+  const void* w;  // or null
+  void* H;        // or null
+  void* Y;
+  float* scales;  // or null
+  int64_t ldx, ldr, ldh, ldy, lds;
+  int64_t M, N;
+  float eps;
+  int w_f32;
+  int group;
+};
+int rms_norm(const RmsNormArgs& p, int dtype, cudaStream_t st);
+
+// ---- dense layer with 4-bit weights (dense_w4.cu)
+struct W4Layout {
+  int64_t K, N;
+  int group;    // columns of K with one scale: 32 or a multiple of 64
+  int s_dtype;  // kF32, kBF16 or kF16
+  bool has_zeros;
+  int64_t kblocks() const { return (K + 63) / 64; }
+  int64_t strips() const { return (N + 63) / 64; }
+  int64_t groups() const { return (K + group - 1) / group; }
+  int64_t codes_bytes() const { return strips() * kblocks() * 2048; }
+  int64_t scales_bytes() const {
+    return (strips() * groups() * 64 * (s_dtype == kF32 ? 4 : 2) + 255) / 256 * 256;
+  }
+  int64_t zeros_bytes() const { return has_zeros ? (strips() * groups() * 64 + 255) / 256 * 256 : 0; }
+  int64_t bytes() const { return codes_bytes() + scales_bytes() + zeros_bytes(); }
+};
+struct DenseW4Args {
+  const void* X;
+  const float* x_scales;  // or null; [M, x_groups], one for each x_group columns (0: the row)
+  const void* packed;
+  const void* b;  // or null
+  void* Y;
+  int64_t ldx, ldxs, ldy, M;
+  W4Layout w;
+  int x_dtype, x_group, b_dtype, y_dtype, act;
+  float alpha;
+};
+int dense_w4(const DenseW4Args& p, cudaStream_t st);
+int w4_quantize(const float* W, int64_t ldw, int64_t K, int64_t N, int group, uint8_t* codes,
+                int64_t ldc, void* scales, int64_t lds, int s_dtype, cudaStream_t st);
+int w4_pack(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds,
+            const uint8_t* zeros, int64_t ldz, const W4Layout& w, void* packed, cudaStream_t st);
+int w4_dequantize(const void* packed, const W4Layout& w, float* W, int64_t ldw, cudaStream_t st);
+
+// ---- token log probabilities (token_logprobs.cu)
+constexpr int kMaxTop = 32;
+struct TokenLogprobsArgs {
+  const void* logits;
+  int64_t ld;
+  int64_t T;
+  int64_t V;
+  const int32_t* tokens;  // or null
+  float* logprobs;        // or null
+  float* entropy;         // or null
+  float* top_logprobs;    // [T, top]
+  int32_t* top_tokens;    // [T, top]
+  int top;
+};
+int token_logprobs(const TokenLogprobsArgs& p, int dtype, cudaStream_t st);
 
 // ---- 1-D reductions / dot (reduce.cu). `y` non-null: dot product (op = sum).
 // `scratch` holds reduce_scratch_bytes(); `out` is one device element.

@@ -1,0 +1,358 @@
+// Root-mean-square norm of rows, with the residual's addition and an output
+// of 8 bits (HBM-bound).
+//
+//   h = x + r                                  (r optional)
+//   y = h / sqrt(mean(h^2) + eps) * w          (w optional)
+//   q = e4m3(y / s),  s = max|y| / 448         over the row or over groups of
+//                                              32, 64 or 128 columns
+//
+// h is summed in f32 and stays there until the end: y comes from the f32 sum,
+// not from the h that is stored in x's type, and q from the f32 y, so each
+// output is rounded once. The sum of squares is a tree over f32 partial sums
+// of at most 32 terms.
+#include <cuda_runtime.h>
+#include <algorithm>
+#include <cstdint>
+#include "dtype.cuh"
+#include "kernels.h"
+
+namespace b200 {
+
+namespace {
+
+constexpr float kE4M3Max = 448.0f;
+// Below this maximum 448 / max leaves the range of f32 (or nears it): the
+// codes are then divided by the scale instead.
+constexpr float kTinyMax = 1e-30f;
+
+struct Sum {
+  static __device__ __forceinline__ float id() { return 0.0f; }
+  static __device__ __forceinline__ float op(float a, float b) { return a + b; }
+};
+struct Max {
+  static __device__ __forceinline__ float id() { return 0.0f; }  // of absolute values
+  static __device__ __forceinline__ float op(float a, float b) { return fmaxf(a, b); }
+};
+
+// Reduction over the TPR threads of a row. For TPR > 32 the CTA is one row;
+// `sh` holds 32 floats and is used by one reduction at a time: the caller
+// alternates between two.
+template <class Op, int TPR>
+__device__ __forceinline__ float row_reduce(float v, float* sh) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = Op::op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if constexpr (TPR > 32) {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < TPR / 32 ? sh[lane] : Op::id();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = Op::op(v, __shfl_xor_sync(0xffffffffu, v, o));
+  }
+  return v;
+}
+
+// Elements [n, n + VEC) of a row as floats, 0 past N.
+template <class T, bool AL>
+__device__ __forceinline__ void load_chunk(const T* row, int64_t n, int64_t N, float* f) {
+  constexpr int VEC = Chunk<T>::kElems;
+  if (AL && n + VEC <= N) {
+    // an ordinary load: h may be stored over x or over the residual
+    unpack(*reinterpret_cast<const uint4*>(row + n), (const T*)nullptr, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = n + i < N ? to_f32(row[n + i]) : 0.0f;
+  }
+}
+
+template <class T, bool AL>
+__device__ __forceinline__ void store_chunk(T* row, int64_t n, int64_t N, const float* f) {
+  constexpr int VEC = Chunk<T>::kElems;
+  if (AL && n + VEC <= N) {
+    *reinterpret_cast<uint4*>(row + n) = pack(f, (const T*)nullptr);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (n + i < N) row[n + i] = from_f32<T>(f[i]);
+  }
+}
+
+// VEC elements of w (T or f32), 1 without one.
+template <class T, bool AL>
+__device__ __forceinline__ void load_weight(const RmsNormArgs& p, int64_t n, float* f) {
+  constexpr int VEC = Chunk<T>::kElems;
+  if (!p.w) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = 1.0f;
+  } else if (sizeof(T) == 4 || !p.w_f32) {
+    load_chunk<T, AL>(static_cast<const T*>(p.w), n, p.N, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4)
+      load_chunk<float, AL>(static_cast<const float*>(p.w), n + i, p.N, f + i);
+  }
+}
+
+// Codes of VEC values with the scale of their row or group.
+template <int VEC, bool AL>
+__device__ __forceinline__ void store_codes(uint8_t* row, int64_t n, int64_t N, const float* y,
+                                            float most, float scale) {
+  float c[VEC];
+  const float inv = kE4M3Max / most;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) c[i] = most > kTinyMax ? y[i] * inv : y[i] / scale;
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4; ++i) {
+    const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(c[4 * i], c[4 * i + 1]),
+                                                __NV_SATFINITE, __NV_E4M3);
+    const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(c[4 * i + 2], c[4 * i + 3]),
+                                                __NV_SATFINITE, __NV_E4M3);
+    w[i] = a | b << 16;
+  }
+  if (AL && n + VEC <= N) {
+    if constexpr (VEC == 8)
+      *reinterpret_cast<uint2*>(row + n) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(row + n) = w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (n + i < N) row[n + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+__device__ __forceinline__ float scale_of(float most) {
+  const float s = most / kE4M3Max;
+  return s > 0.0f ? s : 1.0f;  // nothing but zeros (or underflow): codes of y itself
+}
+
+// The largest of a group's absolute values: the group's lanes are
+// group / VEC consecutive ones.
+__device__ __forceinline__ float group_max(float v, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// y = (h * pre) * inv with inv = 1 / sqrt(mean of squares + eps) and pre = 1.
+// The squares of |h| > 1.8e19 leave f32's range: pre is then 2^-100 and inv
+// that of h * pre (`squares(pre)` sums them over the row again).
+struct Factor {
+  float pre, inv;
+};
+template <class Fn>
+__device__ __forceinline__ Factor factor(float ss, float N, float eps, Fn squares) {
+  if (ss < __int_as_float(0x7f800000)) return {1.0f, 1.0f / sqrtf(ss / N + eps)};
+  const float c = 7.88860905e-31f;
+  return {c, 1.0f / sqrtf(squares(c) / N + eps * c * c)};
+}
+
+// One row by TPR threads, E chunks of 16 bytes a thread: chunk e * TPR + t of
+// the row is thread t's e-th. The row is read once and stays in registers.
+template <class T, int TPR, int E, bool AL>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+    rms_norm_kernel(const __grid_constant__ RmsNormArgs p) {
+  constexpr int VEC = Chunk<T>::kElems;
+  constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
+  __shared__ float sh[3][32];
+  const int t = threadIdx.x % TPR;
+  const int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  if (m >= p.M) return;  // whole warps: TPR is 32 where a CTA has several rows
+  const T* x = static_cast<const T*>(p.X) + m * p.ldx;
+  const T* r = p.R ? static_cast<const T*>(p.R) + m * p.ldr : nullptr;
+
+  float h[E][VEC];
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) load_chunk<T, AL>(x, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
+  if (r) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      float f[VEC];
+      load_chunk<T, AL>(r, (int64_t)(e * TPR + t) * VEC, p.N, f);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[e][i] += f[i];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) ss = fmaf(h[e][i], h[e][i], ss);
+  ss = row_reduce<Sum, TPR>(ss, sh[0]);
+  const Factor f = factor(ss, (float)p.N, p.eps, [&](float c) {
+    float s = 0.0f;
+    for (int e = 0; e < E; ++e)
+      for (int i = 0; i < VEC; ++i) s = fmaf(h[e][i] * c, h[e][i] * c, s);
+    return row_reduce<Sum, TPR>(s, sh[1]);
+  });
+
+  if (p.H) {
+    T* hrow = static_cast<T*>(p.H) + m * p.ldh;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      store_chunk<T, AL>(hrow, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    float w[VEC];
+    load_weight<T, AL>(p, (int64_t)(e * TPR + t) * VEC, w);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) h[e][i] = h[e][i] * f.pre * f.inv * w[i];
+  }
+  if (!p.scales) {
+    T* y = static_cast<T*>(p.Y) + m * p.ldy;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      store_chunk<T, AL>(y, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
+    return;
+  }
+  uint8_t* q = static_cast<uint8_t*>(p.Y) + m * p.ldy;
+  float* s = p.scales + m * p.lds;
+  float most[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    most[e] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) most[e] = fmaxf(most[e], fabsf(h[e][i]));
+  }
+  if (p.group == 0) {
+    float all = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) all = fmaxf(all, most[e]);
+    all = row_reduce<Max, TPR>(all, sh[2]);
+    const float scale = scale_of(all);
+    if (t == 0) s[0] = scale;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      store_codes<VEC, AL>(q, (int64_t)(e * TPR + t) * VEC, p.N, h[e], all, scale);
+  } else {
+    const int lanes = p.group / VEC;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int64_t n = (int64_t)(e * TPR + t) * VEC;
+      const float gm = group_max(most[e], lanes);
+      const float scale = scale_of(gm);
+      if (t % lanes == 0 && n < p.N) s[n / p.group] = scale;
+      store_codes<VEC, AL>(q, n, p.N, h[e], gm, scale);
+    }
+  }
+}
+
+// Rows that do not fit the registers of one CTA: the row is read once for the
+// sum, once more for a row's maximum, and once to be written.
+template <class T, bool AL>
+__global__ void __launch_bounds__(1024)
+    rms_norm_long_kernel(const __grid_constant__ RmsNormArgs p) {
+  constexpr int VEC = Chunk<T>::kElems, TPR = 1024;
+  __shared__ float sh[3][32];
+  const int t = threadIdx.x;
+  const int64_t m = blockIdx.x;
+  const T* x = static_cast<const T*>(p.X) + m * p.ldx;
+  const T* r = p.R ? static_cast<const T*>(p.R) + m * p.ldr : nullptr;
+  const int64_t chunks = (p.N + VEC - 1) / VEC;
+  auto load_h = [&](int64_t c, float* h) {
+    load_chunk<T, AL>(x, c * VEC, p.N, h);
+    if (r) {
+      float f[VEC];
+      load_chunk<T, AL>(r, c * VEC, p.N, f);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[i] += f[i];
+    }
+  };
+  auto squares = [&](float c, float* buf) {
+    float s = 0.0f;
+    for (int64_t j = t; j < chunks; j += TPR) {
+      float h[VEC];
+      load_h(j, h);
+      float part = 0.0f;  // at most VEC terms, then into the thread's sum
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) part = fmaf(h[i] * c, h[i] * c, part);
+      s += part;
+    }
+    return row_reduce<Sum, TPR>(s, buf);
+  };
+  const float ss = squares(1.0f, sh[0]);
+  const Factor f =
+      factor(ss, (float)p.N, p.eps, [&](float c) { return squares(c, sh[1]); });
+  float all = 0.0f, scale = 0.0f;
+  if (p.scales && p.group == 0) {
+    for (int64_t j = t; j < chunks; j += TPR) {
+      float h[VEC], w[VEC];
+      load_h(j, h);
+      load_weight<T, AL>(p, j * VEC, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) all = fmaxf(all, fabsf(h[i] * f.pre * f.inv * w[i]));
+    }
+    all = row_reduce<Max, TPR>(all, sh[2]);
+    scale = scale_of(all);
+    if (t == 0) p.scales[m * p.lds] = scale;
+  }
+  // whole warps take part in every step: a group's lanes exchange their maxima
+  for (int64_t j0 = 0; j0 < chunks; j0 += TPR) {
+    const int64_t n = (j0 + t) * VEC;
+    float h[VEC], w[VEC];
+    load_h(j0 + t, h);
+    load_weight<T, AL>(p, n, w);
+    if (p.H) store_chunk<T, AL>(static_cast<T*>(p.H) + m * p.ldh, n, p.N, h);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) h[i] = h[i] * f.pre * f.inv * w[i];
+    if (!p.scales) {
+      store_chunk<T, AL>(static_cast<T*>(p.Y) + m * p.ldy, n, p.N, h);
+      continue;
+    }
+    float most = all, s = scale;
+    if (p.group) {
+      most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) most = fmaxf(most, fabsf(h[i]));
+      most = group_max(most, p.group / VEC);
+      s = scale_of(most);
+      if (n % p.group == 0 && n < p.N) p.scales[m * p.lds + n / p.group] = s;
+    }
+    store_codes<VEC, AL>(static_cast<uint8_t*>(p.Y) + m * p.ldy, n, p.N, h, most, s);
+  }
+}
+
+template <class T, int TPR, int E, bool AL>
+void launch(const RmsNormArgs& p, cudaStream_t st) {
+  constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
+  rms_norm_kernel<T, TPR, E, AL>
+      <<<(unsigned)((p.M + ROWS - 1) / ROWS), TPR < 128 ? 128 : TPR, 0, st>>>(p);
+}
+
+template <class T, bool AL>
+void dispatch(const RmsNormArgs& p, cudaStream_t st) {
+  const int64_t c = (p.N + Chunk<T>::kElems - 1) / Chunk<T>::kElems;
+  if (c <= 32) launch<T, 32, 1, AL>(p, st);
+  else if (c <= 128) launch<T, 32, 4, AL>(p, st);
+  else if (c <= 256) launch<T, 128, 2, AL>(p, st);
+  else if (c <= 512) launch<T, 256, 2, AL>(p, st);
+  else if (c <= 1024) launch<T, 512, 2, AL>(p, st);
+  else if (c <= 2048) launch<T, 512, 4, AL>(p, st);
+  else if (c <= 4096) launch<T, 1024, 4, AL>(p, st);
+  else rms_norm_long_kernel<T, AL><<<(unsigned)p.M, 1024, 0, st>>>(p);
+}
+
+template <class T>
+void dispatch_aligned(const RmsNormArgs& p, cudaStream_t st) {
+  auto ok = [](const void* q, int64_t ld, int64_t elems, int bytes) {
+    return (reinterpret_cast<uintptr_t>(q) % bytes) == 0 && ld % elems == 0;
+  };
+  constexpr int VEC = Chunk<T>::kElems;
+  const bool al = ok(p.X, p.ldx, VEC, 16) && (!p.R || ok(p.R, p.ldr, VEC, 16)) &&
+                  (!p.H || ok(p.H, p.ldh, VEC, 16)) && (!p.w || ok(p.w, VEC, VEC, 16)) &&
+                  (p.scales ? ok(p.Y, p.ldy, VEC, VEC) : ok(p.Y, p.ldy, VEC, 16));
+  al ? dispatch<T, true>(p, st) : dispatch<T, false>(p, st);
+}
+
+}  // namespace
+
+int rms_norm(const RmsNormArgs& p, int dtype, cudaStream_t st) {
+  if (dtype == kF32) dispatch_aligned<float>(p, st);
+  else if (dtype == kBF16) dispatch_aligned<bf16>(p, st);
+  else dispatch_aligned<f16>(p, st);
+  count_launch();
+  return launch_result();
+}
+
+}  // namespace b200

@@ -22,6 +22,7 @@ ERROR_NAMES = {
 }
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
 REDUCE_SUM, REDUCE_PROD, REDUCE_MAX, REDUCE_MIN = 0, 1, 2, 3
+F32, BF16, F16, E4M3 = 0, 1, 2, 3
 
 # Every symbol include/b200_edsl.h declares (checked by the CPU test-suite).
 EXPORTED_SYMBOLS = [
@@ -47,6 +48,8 @@ EXPORTED_SYMBOLS = [
     "b200_memref_matmul_f32", "b200_memref_matmul_relu_f32", "b200_memref_dense_f32",
     "b200_memref_dense_relu_f32", "b200_memref_matmul_i32", "b200_memref_dense_i32",
     "b200_memref_bias_add_f32", "b200_memref_bias_relu_f32", "b200_memref_relu_f32",
+    "b200_rms_norm", "b200_w4_bytes", "b200_w4_quantize", "b200_w4_pack", "b200_w4_dequantize",
+    "b200_dense_w4", "b200_token_logprobs",
 ]
 
 _lib = None
@@ -130,6 +133,15 @@ def _declare(lib):
         "b200_reduce_i32_host": ([vp, i64, i32, c.c_int32, vp], i32),
         "b200_dot_f32_host": ([vp, vp, i64, vp], i32),
         "b200_dot_i32_host": ([vp, vp, i64, vp], i32),
+        "b200_rms_norm": ([vp, i64, vp, i64, i32, vp, i32, f32, vp, i64, vp, i64, i32, vp, i64,
+                           i32, i64, i64, vp], i32),
+        "b200_w4_bytes": ([i64, i64, i32, i32, i32], i64),
+        "b200_w4_quantize": ([vp, i64, i64, i64, i32, vp, i64, vp, i64, i32, vp], i32),
+        "b200_w4_pack": ([vp, i64, vp, i64, i32, vp, i64, i64, i64, i32, vp, vp], i32),
+        "b200_w4_dequantize": ([vp, i32, i32, i64, i64, i32, vp, i64, vp], i32),
+        "b200_dense_w4": ([vp, i64, i32, vp, i64, i32, vp, i32, i32, i32, vp, i32, vp, i64, i32,
+                           i64, i64, i64, i32, f32, vp], i32),
+        "b200_token_logprobs": ([vp, i64, i32, i64, i64, vp, vp, vp, i32, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)
