@@ -1,16 +1,20 @@
-"""Builds libb200edsl.so (all CUDA kernels + the C-ABI runtime) in-tree.
+"""Builds libb200edsl.so (all CUDA kernels + the C-ABI runtime) and
+b200torch.so (the serving operators' calls on torch tensors) in-tree.
 
 nvcc cross-compiles for sm_100a without a GPU, so this runs on any host with
-the CUDA toolkit. Output: ml-edsl_b200/lib/libb200edsl.so.
+the CUDA toolkit. Output: ml-edsl_b200/lib/.
 """
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libb200edsl.so")
+TORCH_SOURCE = os.path.join(CSRC, "torch_calls.cpp")
+TORCH_LIB = os.path.join(LIBDIR, "b200torch.so")
 SOURCES = ["gemm_tf32x3.cu", "gemm_i32.cu", "gemm_i32_tc.cu", "elementwise.cu", "runtime.cu", "noalloc.cu", "reduce.cu", "peer.cu",
            "rms_norm.cu", "dense_w4.cu", "token_logprobs.cu", "serving.cu"]
 NVCC_FLAGS = [
@@ -29,10 +33,29 @@ def nvcc():
     return "nvcc"
 
 
+def torch_commands():
+    """(compile, link) of the torch module; it finds libb200edsl.so beside it."""
+    import torch
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc())) or "/usr/local/cuda"
+    obj = TORCH_LIB + ".o"
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    include = [os.path.join(base, "include"),
+               os.path.join(base, "include", "torch", "csrc", "api", "include"),
+               os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cxx = os.environ.get("CXX", "g++")
+    compile_ = [cxx, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}"] + \
+        ["-I" + d for d in include] + ["-c", TORCH_SOURCE, "-o", obj]
+    link = [cxx, "-shared", obj, "-o", TORCH_LIB + ".tmp", "-L" + os.path.join(base, "lib"),
+            "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+            "-L" + LIBDIR, "-lb200edsl", "-Wl,-rpath,$ORIGIN"]
+    return compile_, link
+
+
 def needs_build():
-    if not os.path.exists(LIB):
+    if not (os.path.exists(LIB) and os.path.exists(TORCH_LIB)):
         return True
-    t = os.path.getmtime(LIB)
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(HERE, "..", "include", "b200_edsl.h"))
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
@@ -44,10 +67,20 @@ def build(force=False, verbose=False, extra=()):
     os.makedirs(LIBDIR, exist_ok=True)
     cmd = [nvcc()] + NVCC_FLAGS + list(extra) + [os.path.join(CSRC, s) for s in SOURCES] + [
         "-o", LIB + ".tmp", "-lpthread"]
+    compile_, link = torch_commands()
     if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
+        print(" ".join(cmd), " ".join(compile_), " ".join(link), sep="\n")
+    beside = subprocess.Popen(compile_)
+    try:
+        subprocess.run(cmd, check=True)
+    finally:
+        rc = beside.wait()
+    if rc:
+        raise subprocess.CalledProcessError(rc, compile_)
     os.replace(LIB + ".tmp", LIB)
+    subprocess.run(link, check=True)
+    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+    os.remove(TORCH_LIB + ".o")
     return LIB
 
 

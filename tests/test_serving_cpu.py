@@ -158,17 +158,18 @@ def test_python_types_and_devices():
 
 
 def test_rows_of_tensors():
-    rows = serving._rows
-    assert rows(torch.zeros(4, 6), "t") == (4, 6, 6)
-    assert rows(torch.zeros(4, 8)[:, :6], "t") == (4, 6, 8)
-    assert rows(torch.zeros(6), "t") == (1, 6, 6)
-    assert rows(torch.zeros(2, 3, 6), "t") == (6, 6, 6)
-    assert rows(torch.zeros(2, 3, 8)[..., :6], "t") == (6, 6, 8)
-    assert rows(torch.zeros(2, 1, 6).transpose(0, 1), "t") == (2, 6, 6)
-    assert rows(torch.zeros(5, 1)[:, :1], "t") == (5, 1, 1)
-    assert rows(torch.zeros(1, 6).expand(1, 6), "t") == (1, 6, 6)
-    assert rows(torch.zeros(0, 6), "t") == (0, 6, 6)
+    rows = serving._calls.rows_of
+    assert rows(torch.zeros(4, 6)) == (4, 6, 6)
+    assert rows(torch.zeros(4, 8)[:, :6]) == (4, 6, 8)
+    assert rows(torch.zeros(6)) == (1, 6, 6)
+    assert rows(torch.zeros(2, 3, 6)) == (6, 6, 6)
+    assert rows(torch.zeros(2, 3, 8)[..., :6]) == (6, 6, 8)
+    assert rows(torch.zeros(2, 1, 6).transpose(0, 1)) == (2, 6, 6)
+    assert rows(torch.zeros(5, 1)[:, :1]) == (5, 1, 1)
+    assert rows(torch.zeros(1, 6).expand(1, 6)) == (1, 6, 6)
+    assert rows(torch.zeros(0, 6)) == (0, 6, 6)
     for t in (torch.zeros(6, 4).t(), torch.zeros(4, 12)[:, ::2], torch.zeros(1, 6).expand(4, 6),
-              torch.zeros(()), torch.zeros(3, 2, 6).transpose(0, 1)):
+              torch.zeros(()), torch.zeros(3, 2, 6).transpose(0, 1),
+              torch.zeros(1, 2, 6).expand(4, 2, 6)):
         with pytest.raises(ValueError):
-            rows(t, "t")
+            rows(t)
