@@ -30,8 +30,13 @@
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <cstdint>
+#include <cstdlib>
+#include <mutex>
+#include <set>
+#include <utility>
 #include "dtype.cuh"
 #include "kernels.h"
+#include "ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -158,6 +163,13 @@ __global__ void w4_dequantize_kernel(const uint32_t* __restrict__ codes, const c
 
 // ------------------------------------------------------------------ product
 
+// (a & b) | c in one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+
 // The types of the product's operands.
 struct MmaBF16 {
   static constexpr uint32_t kMagic = 0x43004300u;  // 128 + q in bf16: q in the low bits
@@ -174,6 +186,14 @@ struct MmaBF16 {
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4],
+                                                   uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+  }
 };
 struct MmaF16 {
   static constexpr uint32_t kMagic = 0x64006400u;  // 1024 + q in f16
@@ -189,6 +209,14 @@ struct MmaF16 {
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4],
+                                                   uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
   }
 };
 
@@ -327,6 +355,12 @@ struct Params {
   int rows;          // rows of X for each blockIdx.y
   int stage_blocks;  // blocks of K whose activations are staged at once
   int x_aligned;
+  int recv_bytes;    // of shared memory for other CTAs' sums
+  int log_cluster;   // CTAs that share K
+  int group_shift;   // log2 of the group, or -1
+  __device__ __forceinline__ unsigned group_of(int k) const {
+    return group_shift >= 0 ? (unsigned)k >> group_shift : (unsigned)k / (unsigned)a.w.group;
+  }
 };
 
 // A CTA computes WN * MT * 16 columns of Y for `rows` rows of X, over its
@@ -544,6 +578,388 @@ __global__ void __launch_bounds__(kWarps * 32)
   if (C > 1) cluster.sync();  // nobody reads this CTA's shared memory any more
 }
 
+// Lets `kernel` use 200 KB of dynamic shared memory on the current device.
+cudaError_t allow_shared(const void* kernel) {
+  static std::mutex mu;
+  static std::set<std::pair<const void*, int>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lk(mu);
+  if (done.count({kernel, dev})) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e == cudaSuccess) done.insert({kernel, dev});
+  return e;
+}
+
+// Scales and zeros of one block for a lane, as read from memory.
+template <int SUBS>
+struct RawScales {
+  uint4 s[SUBS][2];
+  uint2 z[SUBS];
+};
+
+__device__ __forceinline__ void cp_async16(void* smem, const void* global) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(smem)),
+               "l"(global)
+               : "memory");
+}
+
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
+// Brings `bytes` (a multiple of 16) at a 16-byte aligned address into L2.
+__device__ __forceinline__ void prefetch_l2_bulk(const void* p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
+}
+
+// Few rows: a CTA has one strip of 64 columns and at most 8 * NT operand
+// columns, and its four warps split the blocks of its part of K. Every lane
+// copies the codes that it will use itself, kDepth blocks ahead, into shared
+// memory (cp.async), so the loop over K has no barrier; scales and zeros are
+// one block ahead in registers. The activations of the CTA's part of K are
+// staged once, or stage_blocks of K at a time where that takes more than
+// kXBytes. CTAs are small so that several share an SM and the last wave is
+// short; the CTAs of a cluster share K.
+#ifndef W4MINB
+#define W4MINB 4
+#define W4OCC 4
+#endif
+constexpr int kFewWarps = 4;
+constexpr int kDepth = 4;
+constexpr int kXBytes = 24 * 1024;
+
+template <int XT, int NT, bool FINE>
+__global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
+    dense_w4_few_kernel(const __grid_constant__ Params p) {
+  using X = XRow<XT>;
+  using Mma = typename X::Mma;
+  using T = typename X::T;
+  constexpr int MT = 4, SUBS = FINE ? 2 : 1, THREADS = kFewWarps * 32;
+  extern __shared__ __align__(16) char smem[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int log_c = p.log_cluster, C = 1 << log_c, rank = blockIdx.x & (C - 1);
+  if (C > 1) cluster.barrier_arrive();
+  pdl_trigger();
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const DenseW4Args& a = p.a;
+  const int64_t strip = blockIdx.x >> log_c, n0 = strip * kStripN;
+  const int64_t m0 = (int64_t)blockIdx.y * p.rows;
+  const int mrows = (int)min((int64_t)p.rows, a.M - m0), cols = mrows * X::kParts;
+  const int K = (int)a.w.K, kblocks = (int)p.kblocks;
+  const int b0 = (int)((int64_t)kblocks * rank >> log_c);
+  const int b1 = (int)((int64_t)kblocks * (rank + 1) >> log_c);
+  const bool s32 = a.w.s_dtype == kF32;
+
+  // shared memory: what the cluster's CTAs send, the codes, the activations
+  char* ring = smem + p.recv_bytes;
+  uint4* mine = reinterpret_cast<uint4*>(ring) + wid * (kDepth * 128) + lane;
+  const uint4* codes = p.codes + (strip * kblocks + b0 + wid) * 128 + lane;  // next to fetch
+  int fetched = b0 + wid;
+  const int64_t col0 = strip * p.groups * 64 + g * 8;
+  auto fetch = [&](int slot) {
+    if (fetched < b1) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) cp_async16(mine + slot * 128 + i * 32, codes + i * 32);
+    }
+    codes += kFewWarps * 128;
+    fetched += kFewWarps;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  RawScales<SUBS> raw;
+  auto fetch_scales = [&](int b) {
+#pragma unroll
+    for (int sub = 0; sub < SUBS; ++sub) {
+      const int k = b * kBlockK + sub * 32;
+      if (b >= b1 || (FINE && k >= K)) return;
+      const int64_t at = col0 + (int64_t)p.group_of(k) * 64;
+      const uint4* sp = reinterpret_cast<const uint4*>(p.scales + (s32 ? at * 4 : at * 2));
+      raw.s[sub][0] = __ldg(sp);
+      if (s32) raw.s[sub][1] = __ldg(sp + 1);
+      if (p.zeros) raw.z[sub] = __ldg(reinterpret_cast<const uint2*>(p.zeros + at));
+    }
+  };
+  // What the CTA will read of the weights is contiguous. The previous kernel of
+  // the stream may still run (and may have written them): until pdl_wait they
+  // are only brought into L2.
+  if (tid == 0 && b0 < b1)
+    prefetch_l2_bulk(p.codes + (strip * kblocks + b0) * 128, (uint32_t)min(b1 - b0, 64) * 2048u);
+  if (tid == 32 && b0 < b1) {
+    const int64_t at = strip * p.groups * 64 + (int64_t)p.group_of(b0 * kBlockK) * 64;
+    prefetch_l2(p.scales + (s32 ? at * 4 : at * 2));
+  }
+  pdl_wait();
+
+  // The activations that are staged first are asked for before the weights.
+  int per_row = min(b1 - b0, p.stage_blocks) * 8;  // units of 8 elements
+  const T* xrow = static_cast<const T*>(a.X) + m0 * a.ldx;
+  auto load_x = [&](int s0, int m, int c, T (&e)[8]) {
+    load8(xrow + m * a.ldx, (int64_t)s0 * kBlockK + c * 8, K, p.x_aligned, e);
+  };
+  auto next_unit = [&](int& m, int& c) {
+    while (c >= per_row) {
+      c -= per_row;
+      ++m;
+    }
+  };
+  __align__(16) T first[8];
+  int m = 0, c = tid;
+  if (b0 < b1) {
+    next_unit(m, c);
+    if (m < mrows) load_x(b0, m, c, first);
+  }
+#pragma unroll
+  for (int i = 0; i < kDepth; ++i) fetch(i);
+  fetch_scales(b0 + wid);
+
+  char* xsm = ring + kFewWarps * kDepth * 2048;
+  const int pitch = p.stage_blocks * 128 + 64;  // bytes of a staged column: 64 mod 128
+  float total[MT][NT][4];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) total[i][j][c] = 0.0f;
+
+  int b = b0 + wid, slot = 0;
+  for (int s0 = b0; s0 < b1; s0 += p.stage_blocks) {
+    const int s1 = min(b1, s0 + p.stage_blocks);
+    if (s0 != b0) __syncthreads();
+    if (s0 != b0) {
+      per_row = (s1 - s0) * 8;
+      m = 0;
+      c = tid;
+      next_unit(m, c);
+      if (m < mrows) load_x(s0, m, c, first);
+    }
+    auto store_x = [&](int m, int c, const T (&e)[8]) {
+      uint4 out[X::kParts];
+      X::stage(e, out);
+#pragma unroll
+      for (int q = 0; q < X::kParts; ++q)
+        *reinterpret_cast<uint4*>(xsm + (m * X::kParts + q) * pitch + c * 16) = out[q];
+    };
+    if (m < mrows) store_x(m, c, first);
+    while (m < mrows) {  // the others, four loads at a time
+      constexpr int U = 4;
+      __align__(16) T e[U][8];
+      int um[U], uc[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        c += THREADS;
+        next_unit(m, c);
+        um[u] = m;
+        uc[u] = c;
+        if (m < mrows) load_x(s0, m, c, e[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (um[u] < mrows) store_x(um[u], uc[u], e[u]);
+    }
+    __syncthreads();
+    const char* xs = xsm + g * pitch + (b - s0) * 128 + t * 16;
+    for (; b < s1; b += kFewWarps) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+      const RawScales<SUBS> rs = raw;
+      fetch_scales(b + kFewWarps);
+#pragma unroll
+      for (int sub = 0; sub < SUBS; ++sub) {
+        const int k = b * kBlockK + sub * 32;
+        if (FINE && k >= K) break;  // the second half of the last block
+        uint32_t zero[2 * MT];
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)  // one byte of z under the magic number's
+          zero[i] = p.zeros ? __byte_perm(i < 4 ? rs.z[sub].x : rs.z[sub].y, Mma::kMagic,
+                                          0x5050 | (i & 3) * 0x0101)
+                            : 0x00080008u | Mma::kMagic;
+        float acc[MT][NT][4];
+#pragma unroll
+        for (int h = FINE ? sub : 0; h < (FINE ? sub + 1 : 2); ++h) {
+          uint4 xb[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j)  // columns that no row has are zero
+            xb[j] = j * 8 + g < cols
+                        ? *reinterpret_cast<const uint4*>(xs + j * 8 * pitch + h * 64)
+                        : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const uint2 w = reinterpret_cast<const uint2*>(mine + slot * 128 + i * 32)[h];
+#pragma unroll
+            for (int step = 0; step < 2; ++step) {
+              uint32_t f[4];
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                f[r] = Mma::sub(and_or((step == 0 ? w.x : w.y) >> (4 * r), 0x000f000fu, Mma::kMagic),
+                                zero[2 * i + (r & 1)]);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                const uint32_t b0 = step == 0 ? xb[j].x : xb[j].z;
+                const uint32_t b1 = step == 0 ? xb[j].y : xb[j].w;
+                if (step == 0 && (FINE || h == 0)) Mma::mma_first(acc[i][j], f, b0, b1);
+                else Mma::mma(acc[i][j], f, b0, b1);
+              }
+            }
+          }
+        }
+        // scales of the rows of X, where they have one for each group of K
+        if (XT == kE4M3 && a.x_group > 0) {
+          const unsigned xg = (unsigned)k / (unsigned)a.x_group;
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int m = j * 8 + t * 2 + c;
+              const float s = m < mrows ? __ldg(a.x_scales + (m0 + m) * a.ldxs + xg) : 0.0f;
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                acc[i][j][c] *= s;
+                acc[i][j][2 + c] *= s;
+              }
+            }
+        }
+        float sc[2 * MT];
+        if (s32) {
+          unpack(rs.s[sub][0], (const float*)nullptr, sc);
+          unpack(rs.s[sub][1], (const float*)nullptr, sc + 4);
+        } else if (a.w.s_dtype == kBF16) {
+          unpack(rs.s[sub][0], (const bf16*)nullptr, sc);
+        } else {
+          unpack(rs.s[sub][0], (const f16*)nullptr, sc);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              total[i][j][c] = fmaf(acc[i][j][c], sc[2 * i + (c >> 1)], total[i][j][c]);
+      }
+      fetch(slot);
+      slot = (slot + 1) & (kDepth - 1);
+      xs += kFewWarps * 128;
+    }
+  }
+
+  // ---- add the warps' parts of K in order, then the CTAs'. Each 32 outputs
+  // of a row belong to one CTA of the cluster, in turn: the others send it
+  // their sums.
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(ring);   // [warp][column][64]
+  float* recv = reinterpret_cast<float*>(smem);  // [CTA][part][slot]
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int col = j * 8 + t * 2 + c;
+      if (col < cols) {
+        float* to = red + (wid * NT * 8 + col) * 64 + g;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          to[i * 16] = total[i][j][c];
+          to[i * 16 + 8] = total[i][j][2 + c];
+        }
+      }
+    }
+  __syncthreads();
+  const int outs = mrows * 64;
+  const int slots = ((mrows * 2 + C - 1) >> log_c) * 32;  // outputs of a CTA
+  if (C > 1) cluster.barrier_wait();                     // every CTA of the cluster runs
+  for (int u = tid; u < outs * X::kParts; u += THREADS) {
+    const int col = u >> 6, m = col / X::kParts, q = col - m * X::kParts;
+    float v = red[u];
+#pragma unroll
+    for (int k = 1; k < kFewWarps; ++k) v += red[k * NT * 8 * 64 + u];
+    const int chunk = m * 2 + (u >> 5 & 1);
+    float* dst = recv + (rank * X::kParts + q) * slots + (chunk >> log_c) * 32 + (u & 31);
+    *(C > 1 ? cluster.map_shared_rank(dst, chunk & (C - 1)) : dst) = v;
+  }
+  // the bias of this thread's first output is on its way meanwhile
+  auto bias_of = [&](int u) {
+    const int64_t n = n0 + (((u >> 5 << log_c) + rank) * 32 + (u & 31) & 63);
+    return a.b && n < a.w.N ? load_as_f32(a.b, a.b_dtype, n) : 0.0f;
+  };
+  float bias = bias_of(tid);
+  if (C > 1) cluster.sync();
+  else __syncthreads();
+  for (int u = tid; u < slots; u += THREADS) {
+    if (u != tid) bias = bias_of(u);
+    const int o = ((u >> 5 << log_c) + rank) * 32 + (u & 31), m = o >> 6, n = o & 63;
+    if (o >= outs || n0 + n >= a.w.N) continue;
+    float part[X::kParts];
+#pragma unroll
+    for (int q = 0; q < X::kParts; ++q) part[q] = recv[q * slots + u];
+    for (int r = 1; r < C; ++r)
+#pragma unroll
+      for (int q = 0; q < X::kParts; ++q) part[q] += recv[(r * X::kParts + q) * slots + u];
+    float y = part[X::kParts - 1];  // the smallest part first
+#pragma unroll
+    for (int q = X::kParts - 2; q >= 0; --q) y += part[q];
+    if (a.x_scales && a.x_group == 0) y *= __ldg(a.x_scales + (m0 + m) * a.ldxs);
+    if (a.b) y += bias;
+    y = activate(y, a.act, a.alpha);
+    const int64_t at = (m0 + m) * a.ldy + n0 + n;
+    if (a.y_dtype == kF32) static_cast<float*>(a.Y)[at] = y;
+    else if (a.y_dtype == kBF16) static_cast<bf16*>(a.Y)[at] = __float2bfloat16_rn(y);
+    else static_cast<f16*>(a.Y)[at] = __float2half_rn(y);
+  }
+}
+
+template <int XT, int NT, bool FINE>
+int launch_few(Params p, cudaStream_t st) {
+  auto kernel = dense_w4_few_kernel<XT, NT, FINE>;
+  p.rows = NT * 8 / XRow<XT>::kParts;
+  const int64_t tiles = p.a.w.strips();
+  const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
+  if (chunks > 65535) return kErrTooLarge;
+  // CTAs that share K: the fewest waves of the GPU's 148 * W4OCC CTAs, each as
+  // long as a warp's blocks and kFixed of setting up and adding.
+  constexpr int kFixed = 4;
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int l = 0; l <= 3; ++l) {
+    const int64_t waves = ((tiles * chunks << l) + 148 * W4OCC - 1) / (148 * W4OCC);
+    const int64_t blocks = (p.kblocks + (kFewWarps << l) - 1) / (kFewWarps << l);
+    const int64_t cost = waves * (blocks + kFixed);
+    if (cost < least) {
+      least = cost;
+      best = l;
+    }
+  }
+  static const int force = getenv("W4C") ? atoi(getenv("W4C")) : -1;
+  if (force >= 0) best = force;
+  const int C = 1 << best;
+  p.log_cluster = best;
+  const int64_t mine = (p.kblocks + C - 1) / C;
+  const int rows = (int)std::min<int64_t>(p.rows, p.a.M), cols = rows * XRow<XT>::kParts;
+  p.stage_blocks = (int)std::max<int64_t>(
+      1, std::min<int64_t>(mine, std::max(kFewWarps, (kXBytes / cols - 64) / 128 / kFewWarps *
+                                                         kFewWarps)));
+  p.recv_bytes = C * XRow<XT>::kParts * ((rows * 2 + C - 1) / C * 32) * 4;
+  const int smem = p.recv_bytes + kFewWarps * kDepth * 2048 + cols * (p.stage_blocks * 128 + 64);
+  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel));
+  if (e0 != cudaSuccess) return launch_result(e0);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)chunks);
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = C;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  count_launch();
+  return launch_result(e != cudaSuccess ? e : cudaGetLastError());
+}
+
 template <int XT, int NT, int MT, int WN, bool FINE>
 int launch(Params p, cudaStream_t st) {
   constexpr int WK = kWarps / WN, COLS = NT * 8, ROWS = WN * MT * 16;
@@ -561,15 +977,8 @@ int launch(Params p, cudaStream_t st) {
   p.stage_blocks = (int)std::max<int64_t>(
       WK, std::min<int64_t>((mine + WK - 1) / WK * WK, (kStage / COLS - 64) / 128 / WK * WK));
   const int smem = std::max(COLS * (p.stage_blocks * 128 + 64), WK * COLS * ROWS * 4);
-  static int allowed[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (smem > 48 * 1024 && allowed[dev] < smem) {
-    const cudaError_t e = cudaFuncSetAttribute(
-        kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-    if (e != cudaSuccess) return launch_result(e);
-    allowed[dev] = 200 * 1024;
-  }
+  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel));
+  if (e0 != cudaSuccess) return launch_result(e0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)chunks);
   cfg.blockDim = dim3(kWarps * 32);
@@ -590,8 +999,8 @@ int launch(Params p, cudaStream_t st) {
 template <int XT, bool FINE>
 int dispatch_rows(const Params& p, cudaStream_t st) {
   const int64_t cols = p.a.M * XRow<XT>::kParts;
-  if (cols <= 8) return launch<XT, 1, 4, 1, FINE>(p, st);
-  if (cols <= 16) return launch<XT, 2, 4, 1, FINE>(p, st);
+  if (cols <= 8) return launch_few<XT, 1, FINE>(p, st);
+  if (cols <= 16) return launch_few<XT, 2, FINE>(p, st);
   if (cols <= 32) return launch<XT, 4, 2, 2, FINE>(p, st);
   return launch<XT, 8, 2, 4, FINE>(p, st);
 }
@@ -619,7 +1028,10 @@ int dense_w4(const DenseW4Args& a, cudaStream_t st) {
                 : nullptr;
   p.kblocks = a.w.kblocks();
   p.groups = a.w.groups();
-  p.rows = p.stage_blocks = 0;
+  p.rows = p.stage_blocks = p.recv_bytes = p.log_cluster = 0;
+  p.group_shift = -1;
+  for (int l = 5; l < 31; ++l)
+    if (a.w.group == 1 << l) p.group_shift = l;
   const int64_t bytes = dtype_bytes(a.x_dtype);
   const int64_t unit = a.x_dtype == kE4M3 ? 8 : 16;
   p.x_aligned = reinterpret_cast<uintptr_t>(a.X) % unit == 0 && a.ldx * bytes % unit == 0;
