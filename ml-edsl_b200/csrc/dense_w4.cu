@@ -592,13 +592,6 @@ cudaError_t allow_shared(const void* kernel) {
   return e;
 }
 
-// Scales and zeros of one block for a lane, as read from memory.
-template <int SUBS>
-struct RawScales {
-  uint4 s[SUBS][2];
-  uint2 z[SUBS];
-};
-
 __device__ __forceinline__ void cp_async16(void* smem, const void* global) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(smem)),
                "l"(global)
@@ -668,17 +661,31 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
     fetched += kFewWarps;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  RawScales<SUBS> raw;
+  // a block's scales are asked for when the scales before them have been used,
+  // its zeros one block ahead
+  const char* lane_scales = p.scales + (s32 ? col0 * 4 : col0 * 2);
+  const int scale_step = s32 ? 256 : 128;  // bytes of a group
+  uint4 raw[SUBS][2];
+  uint2 zraw[SUBS];
   auto fetch_scales = [&](int b) {
+    if (b >= b1) return;
 #pragma unroll
     for (int sub = 0; sub < SUBS; ++sub) {
       const int k = b * kBlockK + sub * 32;
-      if (b >= b1 || (FINE && k >= K)) return;
-      const int64_t at = col0 + (int64_t)p.group_of(k) * 64;
-      const uint4* sp = reinterpret_cast<const uint4*>(p.scales + (s32 ? at * 4 : at * 2));
-      raw.s[sub][0] = __ldg(sp);
-      if (s32) raw.s[sub][1] = __ldg(sp + 1);
-      if (p.zeros) raw.z[sub] = __ldg(reinterpret_cast<const uint2*>(p.zeros + at));
+      if (FINE && k >= K) return;
+      const uint4* sp =
+          reinterpret_cast<const uint4*>(lane_scales + (int64_t)p.group_of(k) * scale_step);
+      raw[sub][0] = __ldg(sp);
+      if (s32) raw[sub][1] = __ldg(sp + 1);
+    }
+  };
+  auto fetch_zeros = [&](int b) {
+    if (!p.zeros || b >= b1) return;
+#pragma unroll
+    for (int sub = 0; sub < SUBS; ++sub) {
+      const int k = b * kBlockK + sub * 32;
+      if (FINE && k >= K) return;
+      zraw[sub] = __ldg(reinterpret_cast<const uint2*>(p.zeros + col0 + (int64_t)p.group_of(k) * 64));
     }
   };
   // What the CTA will read of the weights is contiguous. The previous kernel of
@@ -713,9 +720,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
 #pragma unroll
   for (int i = 0; i < kDepth; ++i) fetch(i);
   fetch_scales(b0 + wid);
+  fetch_zeros(b0 + wid);
 
   char* xsm = ring + kFewWarps * kDepth * 2048;
   const int pitch = p.stage_blocks * 128 + 64;  // bytes of a staged column: 64 mod 128
+  if (cols < NT * 8 && tid < 8)
+    *reinterpret_cast<uint4*>(xsm + cols * pitch + tid * 16) = make_uint4(0, 0, 0, 0);
   float total[MT][NT][4];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -760,40 +770,49 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
         if (um[u] < mrows) store_x(um[u], uc[u], e[u]);
     }
     __syncthreads();
-    const char* xs = xsm + g * pitch + (b - s0) * 128 + t * 16;
+    // operand column j * 8 + g; columns that no row has read zeros
+    const char* xs[NT];
+    int xstep[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const bool is = j * 8 + g < cols;
+      xs[j] = is ? xsm + (j * 8 + g) * pitch + (b - s0) * 128 + t * 16 : xsm + cols * pitch;
+      xstep[j] = is ? kFewWarps * 128 : 0;
+    }
     for (; b < s1; b += kFewWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
-      const RawScales<SUBS> rs = raw;
-      fetch_scales(b + kFewWarps);
+      uint4 cur[MT];
+#pragma unroll
+      for (int i = 0; i < MT; ++i) cur[i] = mine[slot * 128 + i * 32];
+      uint32_t zero[SUBS][2 * MT];
+#pragma unroll
+      for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i)  // one byte of z under the magic number's
+          zero[sub][i] = p.zeros ? __byte_perm(i < 4 ? zraw[sub].x : zraw[sub].y, Mma::kMagic,
+                                               0x5050 | (i & 3) * 0x0101)
+                                 : 0x00080008u | Mma::kMagic;
+      fetch_zeros(b + kFewWarps);
 #pragma unroll
       for (int sub = 0; sub < SUBS; ++sub) {
         const int k = b * kBlockK + sub * 32;
         if (FINE && k >= K) break;  // the second half of the last block
-        uint32_t zero[2 * MT];
-#pragma unroll
-        for (int i = 0; i < 2 * MT; ++i)  // one byte of z under the magic number's
-          zero[i] = p.zeros ? __byte_perm(i < 4 ? rs.z[sub].x : rs.z[sub].y, Mma::kMagic,
-                                          0x5050 | (i & 3) * 0x0101)
-                            : 0x00080008u | Mma::kMagic;
         float acc[MT][NT][4];
 #pragma unroll
         for (int h = FINE ? sub : 0; h < (FINE ? sub + 1 : 2); ++h) {
           uint4 xb[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j)  // columns that no row has are zero
-            xb[j] = j * 8 + g < cols
-                        ? *reinterpret_cast<const uint4*>(xs + j * 8 * pitch + h * 64)
-                        : make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < NT; ++j) xb[j] = *reinterpret_cast<const uint4*>(xs[j] + h * 64);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
-            const uint2 w = reinterpret_cast<const uint2*>(mine + slot * 128 + i * 32)[h];
+            const uint2 w = h == 0 ? make_uint2(cur[i].x, cur[i].y) : make_uint2(cur[i].z, cur[i].w);
 #pragma unroll
             for (int step = 0; step < 2; ++step) {
               uint32_t f[4];
 #pragma unroll
               for (int r = 0; r < 4; ++r)
                 f[r] = Mma::sub(and_or((step == 0 ? w.x : w.y) >> (4 * r), 0x000f000fu, Mma::kMagic),
-                                zero[2 * i + (r & 1)]);
+                                zero[sub][2 * i + (r & 1)]);
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
                 const uint32_t b0 = step == 0 ? xb[j].x : xb[j].z;
@@ -822,12 +841,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
         }
         float sc[2 * MT];
         if (s32) {
-          unpack(rs.s[sub][0], (const float*)nullptr, sc);
-          unpack(rs.s[sub][1], (const float*)nullptr, sc + 4);
+          unpack(raw[sub][0], (const float*)nullptr, sc);
+          unpack(raw[sub][1], (const float*)nullptr, sc + 4);
         } else if (a.w.s_dtype == kBF16) {
-          unpack(rs.s[sub][0], (const bf16*)nullptr, sc);
+          unpack(raw[sub][0], (const bf16*)nullptr, sc);
         } else {
-          unpack(rs.s[sub][0], (const f16*)nullptr, sc);
+          unpack(raw[sub][0], (const f16*)nullptr, sc);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -837,9 +856,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
             for (int c = 0; c < 4; ++c)
               total[i][j][c] = fmaf(acc[i][j][c], sc[2 * i + (c >> 1)], total[i][j][c]);
       }
+      fetch_scales(b + kFewWarps);
       fetch(slot);
       slot = (slot + 1) & (kDepth - 1);
-      xs += kFewWarps * 128;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) xs[j] += xstep[j];
     }
   }
 
@@ -938,7 +959,8 @@ int launch_few(Params p, cudaStream_t st) {
       1, std::min<int64_t>(mine, std::max(kFewWarps, (kXBytes / cols - 64) / 128 / kFewWarps *
                                                          kFewWarps)));
   p.recv_bytes = C * XRow<XT>::kParts * ((rows * 2 + C - 1) / C * 32) * 4;
-  const int smem = p.recv_bytes + kFewWarps * kDepth * 2048 + cols * (p.stage_blocks * 128 + 64);
+  const int smem = p.recv_bytes + kFewWarps * kDepth * 2048 + cols * (p.stage_blocks * 128 + 64) +
+                   128;  // and the zeros of columns that no row has
   const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel));
   if (e0 != cudaSuccess) return launch_result(e0);
   cudaLaunchConfig_t cfg = {};
