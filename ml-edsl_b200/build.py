@@ -16,7 +16,7 @@ LIB = os.path.join(LIBDIR, "libb200edsl.so")
 TORCH_SOURCE = os.path.join(CSRC, "torch_calls.cpp")
 TORCH_LIB = os.path.join(LIBDIR, "b200torch.so")
 SOURCES = ["gemm_tf32x3.cu", "gemm_i32.cu", "gemm_i32_tc.cu", "elementwise.cu", "runtime.cu", "noalloc.cu", "reduce.cu", "peer.cu",
-           "rms_norm.cu", "dense_w4.cu", "token_logprobs.cu", "serving.cu"]
+           "rms_norm.cu", "dense_w4.cu", "dense_w4_tc.cu", "token_logprobs.cu", "serving.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",

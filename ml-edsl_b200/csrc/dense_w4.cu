@@ -31,23 +31,24 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstdlib>
-#include <mutex>
-#include <set>
-#include <utility>
-#include "dtype.cuh"
-#include "kernels.h"
-#include "ptx.cuh"
+#include "w4.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace b200 {
 
-namespace {
+cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (allowed.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
-constexpr int kBlockK = 64;   // k of one packed block
-constexpr int kStripN = 64;   // columns of one strip
-constexpr int kWarps = 8;
-constexpr int kMaxCluster = 8;
+namespace {
 
 // ------------------------------------------------------------------ packing
 
@@ -78,10 +79,6 @@ __global__ void w4_pack_codes_kernel(const uint8_t* __restrict__ codes, int64_t 
     out[i] = w;
   }
 }
-
-// Place of column n (within its strip) among a group's 64 scales or zeros:
-// lane group g = n % 8 reads its eight values together.
-__host__ __device__ __forceinline__ int column_place(int n) { return (n & 7) * 8 + (n >> 3); }
 
 __global__ void w4_pack_columns_kernel(const void* __restrict__ in, int64_t ldi, int64_t groups,
                                        int64_t N, int64_t strips, int bytes,
@@ -163,450 +160,6 @@ __global__ void w4_dequantize_kernel(const uint32_t* __restrict__ codes, const c
 
 // ------------------------------------------------------------------ product
 
-// (a & b) | c in one instruction.
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-
-// The types of the product's operands.
-struct MmaBF16 {
-  static constexpr uint32_t kMagic = 0x43004300u;  // 128 + q in bf16: q in the low bits
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
-                                     *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                             uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4],
-                                                   uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-  }
-};
-struct MmaF16 {
-  static constexpr uint32_t kMagic = 0x64006400u;  // 1024 + q in f16
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a),
-                              *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                             uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4],
-                                                   uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%10,%10,%10,%10};"
-        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
-  }
-};
-
-// How rows of X become operand columns: kParts columns for a row. stage()
-// takes 8 consecutive elements and gives 16 bytes for each column.
-template <int XT>
-struct XRow;
-template <>
-struct XRow<kBF16> {
-  using Mma = MmaBF16;
-  using T = uint16_t;
-  static constexpr int kParts = 1;
-  static __device__ __forceinline__ void stage(const T (&e)[8], uint4 (&out)[1]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
-    out[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <>
-struct XRow<kF16> : XRow<kBF16> {
-  using Mma = MmaF16;
-};
-template <>
-struct XRow<kE4M3> {
-  using Mma = MmaF16;
-  using T = uint8_t;
-  static constexpr int kParts = 1;
-  static __device__ __forceinline__ void stage(const T (&e)[8], uint4 (&out)[1]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-          (__nv_fp8x2_storage_t)(e[2 * i] | (uint16_t)e[2 * i + 1] << 8), __NV_E4M3);
-      w[i] = h.x | (uint32_t)h.y << 16;
-    }
-    out[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-};
-template <>
-struct XRow<kF32> {
-  using Mma = MmaBF16;
-  using T = uint32_t;
-  static constexpr int kParts = 3;
-  // x = hi + mid + lo, each the leading 8 bits of what is left (cut, so that
-  // no part rounds up out of range). Infinities and NaN travel in hi.
-  static __device__ __forceinline__ void stage(const T (&e)[8], uint4 (&out)[3]) {
-    uint32_t p[3][8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool finite = (e[i] & 0x7f800000u) != 0x7f800000u;
-      const bool nan = !finite && (e[i] & 0x007fffffu);
-      p[0][i] = nan ? 0x7fc0u : e[i] >> 16;
-      const float r = __uint_as_float(e[i]) - __uint_as_float(e[i] & 0xffff0000u);
-      const uint32_t rb = __float_as_uint(r) & 0xffff0000u;
-      p[1][i] = finite ? rb >> 16 : 0u;
-      p[2][i] = finite ? __float_as_uint(r - __uint_as_float(rb)) >> 16 : 0u;
-    }
-#pragma unroll
-    for (int q = 0; q < 3; ++q) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = p[q][2 * i] | p[q][2 * i + 1] << 16;
-      out[q] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  }
-};
-
-// Eight elements of a row of X from column k on, 0 from `end` on.
-template <class T>
-__device__ __forceinline__ void load8(const T* row, int64_t k, int64_t end, bool aligned,
-                                      T (&e)[8]) {
-  if (aligned && k + 8 <= end) {
-    if constexpr (sizeof(T) == 1) {
-      *reinterpret_cast<uint2*>(e) = __ldg(reinterpret_cast<const uint2*>(row + k));
-    } else {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(row + k) + i);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = k + i < end ? __ldg(row + k + i) : T(0);
-  }
-}
-
-__device__ __forceinline__ float activate(float x, int act, float alpha) {
-  if (act == kActRelu) return (x > 0.0f || x != x) ? x : 0.0f;
-  if (act == kActLeakyRelu) {
-    const float pos = (x > 0.0f || x != x) ? x : 0.0f;
-    const float neg = (x < 0.0f || x != x) ? x : 0.0f;
-    return pos + neg * alpha;
-  }
-  return x;
-}
-
-// Eight scales of a lane as floats: scale of fragment row `half` of 16-column
-// piece mt is v[2 * mt + half].
-template <int MT>
-__device__ __forceinline__ void load_scales(const char* p, int s_dtype, float (&v)[2 * MT]) {
-  if (s_dtype == kF32) {
-#pragma unroll
-    for (int i = 0; i < MT / 2; ++i) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
-      v[4 * i] = f.x;
-      v[4 * i + 1] = f.y;
-      v[4 * i + 2] = f.z;
-      v[4 * i + 3] = f.w;
-    }
-    return;
-  }
-  uint32_t w[MT];
-  if constexpr (MT == 4)
-    *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
-  else
-    *reinterpret_cast<uint2*>(w) = __ldg(reinterpret_cast<const uint2*>(p));
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    if (s_dtype == kBF16) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    } else {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x;
-      v[2 * i + 1] = f.y;
-    }
-  }
-}
-
-struct Params {
-  DenseW4Args a;
-  const uint4* codes;
-  const char* scales;
-  const uint8_t* zeros;
-  int64_t kblocks, groups;
-  int rows;          // rows of X for each blockIdx.y
-  int stage_blocks;  // blocks of K whose activations are staged at once
-  int x_aligned;
-  int recv_bytes;    // of shared memory for other CTAs' sums
-  int log_cluster;   // CTAs that share K
-  int group_shift;   // log2 of the group, or -1
-  __device__ __forceinline__ unsigned group_of(int k) const {
-    return group_shift >= 0 ? (unsigned)k >> group_shift : (unsigned)k / (unsigned)a.w.group;
-  }
-};
-
-// A CTA computes WN * MT * 16 columns of Y for `rows` rows of X, over its
-// part of K (the CTAs of a cluster share K): WN warps side by side in N, the
-// others of the eight split the blocks of K among them. Each warp keeps the
-// next block's codes in flight in registers. The parts of K are added in
-// shared memory, warps first, then the cluster's CTAs, in a fixed order.
-template <int XT, int NT, int MT, int WN, bool FINE>
-__global__ void __launch_bounds__(kWarps * 32)
-    dense_w4_kernel(const __grid_constant__ Params p) {
-  using X = XRow<XT>;
-  using Mma = typename X::Mma;
-  using T = typename X::T;
-  constexpr int WK = kWarps / WN, COLS = NT * 8, ROWS = WN * MT * 16;
-  constexpr int SUBS = FINE ? 2 : 1;  // scales applied every 32 or every 64 of K
-  extern __shared__ __align__(16) char smem[];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int wn = wid % WN, wk = wid / WN;
-  const DenseW4Args& a = p.a;
-  const int64_t n0 = (int64_t)(blockIdx.x / C) * ROWS;
-  const int64_t m0 = (int64_t)blockIdx.y * p.rows;
-  const int mrows = (int)min((int64_t)p.rows, a.M - m0);
-  // blocks of K of this CTA
-  const int K = (int)a.w.K, kblocks = (int)p.kblocks;
-  const int b0 = (int)((int64_t)kblocks * rank / C), b1 = (int)((int64_t)kblocks * (rank + 1) / C);
-  // this warp's 16-column pieces: MT of the four of a strip
-  const int64_t nw = n0 + (int64_t)wn * MT * 16;
-  const int64_t strip = nw / kStripN;
-  const int mt0 = (int)(nw % kStripN) / 16;
-  const bool live = nw < a.w.N;  // the last CTA may have warps past the last strip
-  const uint4* codes = p.codes + (strip * p.kblocks * 4 + mt0) * 32 + lane;
-  const int64_t col0 = strip * p.groups * 64 + g * 8 + mt0 * 2;
-  const int sbytes = a.w.s_dtype == kF32 ? 4 : 2;
-
-  const int pitch = p.stage_blocks * 128 + 64;  // bytes of a staged column: 64 mod 128
-  float total[MT][NT][4];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) total[i][j][c] = 0.0f;
-
-  uint4 next[MT];
-  auto fetch = [&](int b) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-      next[i] = live && b < b1 ? __ldcs(codes + (int64_t)b * 128 + i * 32) : make_uint4(0, 0, 0, 0);
-  };
-  int b = b0 + wk;
-  fetch(b);
-
-  for (int s0 = b0; s0 < b1; s0 += p.stage_blocks) {
-    const int s1 = min(b1, s0 + p.stage_blocks);
-    // ---- stage the activations of blocks [s0, s1): column m * parts + part
-    const int per_row = (s1 - s0) * 8;  // units of 8 elements
-    if (s0 != b0) __syncthreads();
-    for (int u = tid; u < per_row * (COLS / X::kParts); u += kWarps * 32) {
-      const int m = u / per_row, c = u - m * per_row;
-      uint4 out[X::kParts];
-      if (m < mrows) {
-        __align__(16) T e[8];
-        load8(static_cast<const T*>(a.X) + (m0 + m) * a.ldx, (int64_t)s0 * kBlockK + c * 8, K,
-              p.x_aligned, e);
-        X::stage(e, out);
-      } else {
-#pragma unroll
-        for (int q = 0; q < X::kParts; ++q) out[q] = make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int q = 0; q < X::kParts; ++q)
-        *reinterpret_cast<uint4*>(smem + (m * X::kParts + q) * pitch + c * 16) = out[q];
-    }
-    if (X::kParts > 1)  // columns that no row has
-      for (int u = tid; u < per_row * (COLS % X::kParts); u += kWarps * 32) {
-        const int q = COLS - COLS % X::kParts + u / per_row;
-        *reinterpret_cast<uint4*>(smem + q * pitch + u % per_row * 16) = make_uint4(0, 0, 0, 0);
-      }
-    __syncthreads();
-
-    for (; b < s1; b += WK) {
-      uint4 cur[MT];
-#pragma unroll
-      for (int i = 0; i < MT; ++i) cur[i] = next[i];
-      fetch(b + WK);
-      if (!live) continue;
-      const char* xs = smem + g * pitch + (b - s0) * 128 + t * 16;
-#pragma unroll
-      for (int sub = 0; sub < SUBS; ++sub) {
-        const int k = b * kBlockK + sub * 32;
-        if (FINE && k >= K) break;  // the second half of the last block
-        const int64_t at = col0 + (int64_t)((unsigned)k / (unsigned)a.w.group) * 64;
-        float sc[2 * MT];
-        load_scales<MT>(p.scales + at * sbytes, a.w.s_dtype, sc);
-        uint32_t zero[2 * MT];
-        if (p.zeros) {
-          uint32_t z[2];
-          if constexpr (MT == 4) {
-            *reinterpret_cast<uint2*>(z) = __ldg(reinterpret_cast<const uint2*>(p.zeros + at));
-          } else {
-            z[0] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
-          }
-#pragma unroll
-          for (int i = 0; i < 2 * MT; ++i)
-            zero[i] = ((z[i >> 2] >> (8 * (i & 3)) & 15u) * 0x00010001u) | Mma::kMagic;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2 * MT; ++i) zero[i] = 0x00080008u | Mma::kMagic;
-        }
-        float acc[MT][NT][4];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.0f;
-#pragma unroll
-        for (int h = FINE ? sub : 0; h < (FINE ? sub + 1 : 2); ++h) {
-          uint4 xb[NT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-            xb[j] = *reinterpret_cast<const uint4*>(xs + j * 8 * pitch + h * 64);
-#pragma unroll
-          for (int step = 0; step < 2; ++step)
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const uint32_t w = h == 0 ? (step == 0 ? cur[i].x : cur[i].y)
-                                        : (step == 0 ? cur[i].z : cur[i].w);
-              uint32_t f[4];
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                f[r] = Mma::sub((w >> (4 * r) & 0x000f000fu) | Mma::kMagic, zero[2 * i + (r & 1)]);
-#pragma unroll
-              for (int j = 0; j < NT; ++j)
-                Mma::mma(acc[i][j], f, step == 0 ? xb[j].x : xb[j].z,
-                         step == 0 ? xb[j].y : xb[j].w);
-            }
-        }
-        // scales of the rows of X, where they have one for each group of K
-        if (XT == kE4M3 && a.x_group > 0) {
-          const unsigned xg = (unsigned)k / (unsigned)a.x_group;
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int m = j * 8 + t * 2 + c;
-              const float s = m < mrows ? __ldg(a.x_scales + (m0 + m) * a.ldxs + xg) : 0.0f;
-#pragma unroll
-              for (int i = 0; i < MT; ++i) {
-                acc[i][j][c] *= s;
-                acc[i][j][2 + c] *= s;
-              }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              total[i][j][c] = fmaf(acc[i][j][c], sc[2 * i + (c >> 1)], total[i][j][c]);
-      }
-    }
-  }
-
-  // ---- add the warps' parts of K, then the CTAs', in shared memory
-  __syncthreads();
-  float* red = reinterpret_cast<float*>(smem);  // [WK][COLS][ROWS]
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        red[(wk * COLS + j * 8 + t * 2 + (c & 1)) * ROWS + wn * MT * 16 + i * 16 + (c >> 1) * 8 +
-            g] = total[i][j][c];
-  __syncthreads();
-  const int cols = mrows * X::kParts;
-  if (WK > 1) {
-    for (int u = tid; u < cols * ROWS; u += kWarps * 32) {
-      float v = red[u];
-#pragma unroll
-      for (int k = 1; k < WK; ++k) v += red[k * COLS * ROWS + u];
-      red[u] = v;
-    }
-    if (C == 1) __syncthreads();
-  }
-  if (C > 1) cluster.sync();
-  const int outs = mrows * ROWS;
-  for (int u = rank * kWarps * 32 + tid; u < outs; u += C * kWarps * 32) {
-    const int m = u / ROWS, n = u - m * ROWS;
-    if (n0 + n >= a.w.N) continue;
-    float part[X::kParts];
-#pragma unroll
-    for (int q = 0; q < X::kParts; ++q) part[q] = 0.0f;
-    for (int r = 0; r < C; ++r) {
-      const float* from = C > 1 ? cluster.map_shared_rank(red, r) : red;
-#pragma unroll
-      for (int q = 0; q < X::kParts; ++q) part[q] += from[(m * X::kParts + q) * ROWS + n];
-    }
-    float y = part[X::kParts - 1];  // the smallest part first
-#pragma unroll
-    for (int q = X::kParts - 2; q >= 0; --q) y += part[q];
-    if (a.x_scales && a.x_group == 0) y *= __ldg(a.x_scales + (m0 + m) * a.ldxs);
-    if (a.b) y += load_as_f32(a.b, a.b_dtype, n0 + n);
-    y = activate(y, a.act, a.alpha);
-    const int64_t at = (m0 + m) * a.ldy + n0 + n;
-    if (a.y_dtype == kF32) static_cast<float*>(a.Y)[at] = y;
-    else if (a.y_dtype == kBF16) static_cast<bf16*>(a.Y)[at] = __float2bfloat16_rn(y);
-    else static_cast<f16*>(a.Y)[at] = __float2half_rn(y);
-  }
-  if (C > 1) cluster.sync();  // nobody reads this CTA's shared memory any more
-}
-
-// Lets `kernel` use 200 KB of dynamic shared memory on the current device.
-cudaError_t allow_shared(const void* kernel) {
-  static std::mutex mu;
-  static std::set<std::pair<const void*, int>> done;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return e;
-  std::lock_guard<std::mutex> lk(mu);
-  if (done.count({kernel, dev})) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
-  if (e == cudaSuccess) done.insert({kernel, dev});
-  return e;
-}
-
-__device__ __forceinline__ void cp_async16(void* smem, const void* global) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(smem)),
-               "l"(global)
-               : "memory");
-}
-
-__device__ __forceinline__ void prefetch_l2(const void* p) {
-  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
-}
-
-// Brings `bytes` (a multiple of 16) at a 16-byte aligned address into L2.
-__device__ __forceinline__ void prefetch_l2_bulk(const void* p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
-}
-
 // Few rows: a CTA has one strip of 64 columns and at most 8 * NT operand
 // columns, and its four warps split the blocks of its part of K. Every lane
 // copies the codes that it will use itself, kDepth blocks ahead, into shared
@@ -625,7 +178,7 @@ constexpr int kXBytes = 24 * 1024;
 
 template <int XT, int NT, bool FINE>
 __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
-    dense_w4_few_kernel(const __grid_constant__ Params p) {
+    dense_w4_few_kernel(const __grid_constant__ W4Params p) {
   using X = XRow<XT>;
   using Mma = typename X::Mma;
   using T = typename X::T;
@@ -929,7 +482,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
 }
 
 template <int XT, int NT, bool FINE>
-int launch_few(Params p, cudaStream_t st) {
+int launch_few(W4Params p, cudaStream_t st) {
   auto kernel = dense_w4_few_kernel<XT, NT, FINE>;
   p.rows = NT * 8 / XRow<XT>::kParts;
   const int64_t tiles = p.a.w.strips();
@@ -961,7 +514,8 @@ int launch_few(Params p, cudaStream_t st) {
   p.recv_bytes = C * XRow<XT>::kParts * ((rows * 2 + C - 1) / C * 32) * 4;
   const int smem = p.recv_bytes + kFewWarps * kDepth * 2048 + cols * (p.stage_blocks * 128 + 64) +
                    128;  // and the zeros of columns that no row has
-  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel));
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
   if (e0 != cudaSuccess) return launch_result(e0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)chunks);
@@ -982,55 +536,14 @@ int launch_few(Params p, cudaStream_t st) {
   return launch_result(e != cudaSuccess ? e : cudaGetLastError());
 }
 
-template <int XT, int NT, int MT, int WN, bool FINE>
-int launch(Params p, cudaStream_t st) {
-  constexpr int WK = kWarps / WN, COLS = NT * 8, ROWS = WN * MT * 16;
-  auto kernel = dense_w4_kernel<XT, NT, MT, WN, FINE>;
-  p.rows = COLS / XRow<XT>::kParts;
-  const int64_t tiles = (p.a.w.N + ROWS - 1) / ROWS;
-  const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
-  if (chunks > 65535) return kErrTooLarge;
-  // K is shared by the CTAs of a cluster until they fill the GPU twice or a
-  // warp has less than one block of K.
-  int C = 1;
-  while (C < kMaxCluster && tiles * chunks * C < 148 * 2 && p.kblocks >= (int64_t)2 * C * WK) C *= 2;
-  constexpr int kStage = 64 * 1024;
-  const int64_t mine = (p.kblocks + C - 1) / C;
-  p.stage_blocks = (int)std::max<int64_t>(
-      WK, std::min<int64_t>((mine + WK - 1) / WK * WK, (kStage / COLS - 64) / 128 / WK * WK));
-  const int smem = std::max(COLS * (p.stage_blocks * 128 + 64), WK * COLS * ROWS * 4);
-  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel));
-  if (e0 != cudaSuccess) return launch_result(e0);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)chunks);
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
-  count_launch();
-  return launch_result(e != cudaSuccess ? e : cudaGetLastError());
-}
-
-template <int XT, bool FINE>
-int dispatch_rows(const Params& p, cudaStream_t st) {
-  const int64_t cols = p.a.M * XRow<XT>::kParts;
-  if (cols <= 8) return launch_few<XT, 1, FINE>(p, st);
-  if (cols <= 16) return launch_few<XT, 2, FINE>(p, st);
-  if (cols <= 32) return launch<XT, 4, 2, 2, FINE>(p, st);
-  return launch<XT, 8, 2, 4, FINE>(p, st);
-}
-
 template <int XT>
-int dispatch(const Params& p, cudaStream_t st) {
+int dispatch(const W4Params& p, int* status, cudaStream_t st) {
   const bool fine = p.a.w.group == 32 || p.a.x_group == 32;
-  return fine ? dispatch_rows<XT, true>(p, st) : dispatch_rows<XT, false>(p, st);
+  const int64_t cols = p.a.M * XRow<XT>::kParts;
+  static const int most = getenv("W4MOST") ? atoi(getenv("W4MOST")) : 8;
+  if (cols > most) return dense_w4_tc(p, status, st);
+  if (cols <= 8) return fine ? launch_few<XT, 1, true>(p, st) : launch_few<XT, 1, false>(p, st);
+  return fine ? launch_few<XT, 2, true>(p, st) : launch_few<XT, 2, false>(p, st);
 }
 
 unsigned grid_for(int64_t work) {
@@ -1039,8 +552,8 @@ unsigned grid_for(int64_t work) {
 
 }  // namespace
 
-int dense_w4(const DenseW4Args& a, cudaStream_t st) {
-  Params p;
+int dense_w4(const DenseW4Args& a, int* status, cudaStream_t st) {
+  W4Params p;
   p.a = a;
   const char* base = static_cast<const char*>(a.packed);
   p.codes = reinterpret_cast<const uint4*>(base);
@@ -1058,10 +571,10 @@ int dense_w4(const DenseW4Args& a, cudaStream_t st) {
   const int64_t unit = a.x_dtype == kE4M3 ? 8 : 16;
   p.x_aligned = reinterpret_cast<uintptr_t>(a.X) % unit == 0 && a.ldx * bytes % unit == 0;
   switch (a.x_dtype) {
-    case kF32: return dispatch<kF32>(p, st);
-    case kBF16: return dispatch<kBF16>(p, st);
-    case kF16: return dispatch<kF16>(p, st);
-    default: return dispatch<kE4M3>(p, st);
+    case kF32: return dispatch<kF32>(p, status, st);
+    case kBF16: return dispatch<kBF16>(p, status, st);
+    case kF16: return dispatch<kF16>(p, status, st);
+    default: return dispatch<kE4M3>(p, status, st);
   }
 }
 

@@ -30,6 +30,10 @@ void count_launch();
 int report_error(int code, const char* msg);
 int report_ok();
 
+// The current device's status word (see check of b200_stream_sync), or an
+// error code. Makes the device's context on its first call.
+int device_status_word(int** out);
+
 // Status of the kernel launch just queued on this thread: kOk, or kErrCuda
 // with the CUDA error's text kept for launch_error_text() (the error is
 // cleared). driver_failure() keeps the text of a failed driver call (tensor
@@ -209,7 +213,7 @@ struct DenseW4Args {
   int x_dtype, x_group, b_dtype, y_dtype, act;
   float alpha;
 };
-int dense_w4(const DenseW4Args& p, cudaStream_t st);
+int dense_w4(const DenseW4Args& p, int* status, cudaStream_t st);
 int w4_quantize(const float* W, int64_t ldw, int64_t K, int64_t N, int group, uint8_t* codes,
                 int64_t ldc, void* scales, int64_t lds, int s_dtype, cudaStream_t st);
 int w4_pack(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds,

@@ -970,6 +970,13 @@ int reduce_device_impl(const T* x, const T* y, int64_t n, int op, T init, T* out
 int report_error(int code, const char* msg) { return fail(code, msg); }
 int report_ok() { return succeed(); }
 
+int device_status_word(int** out) {
+  DeviceCtx* c = nullptr;
+  const int rc = current_ctx(&c);
+  if (rc == kOk) *out = c->status;
+  return rc;
+}
+
 namespace {
 thread_local std::string t_launch_err;
 }

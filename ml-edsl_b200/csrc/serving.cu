@@ -130,6 +130,9 @@ int b200_w4_pack(const uint8_t* codes, int64_t ldc, const void* scales, int64_t 
     return bad("null buffer or pitch < N");
   if (misplaced(scales, s_dtype)) return bad("buffer not aligned to its element type");
   if (unaligned16(packed)) return bad("packed weights must be 16-byte aligned");
+  // the device's context is made here, so that b200_dense_w4 can be captured
+  int* status = nullptr;
+  if (const int rc = device_status_word(&status)) return rc;
   return done(w4_pack(codes, ldc, scales, lds, zeros, ldz,
                       w4_layout(K, N, group, s_dtype, zeros != nullptr), packed,
                       static_cast<cudaStream_t>(stream)),
@@ -188,7 +191,9 @@ int b200_dense_w4(const void* X, int64_t ldx, int x_dtype, const float* x_scales
   p.y_dtype = y_dtype;
   p.act = act;
   p.alpha = alpha;
-  return done(dense_w4(p, static_cast<cudaStream_t>(stream)), "dense_w4");
+  int* status = nullptr;
+  if (const int rc = device_status_word(&status)) return rc;
+  return done(dense_w4(p, status, static_cast<cudaStream_t>(stream)), "dense_w4");
 }
 
 int b200_token_logprobs(const void* logits, int64_t ld, int dtype, int64_t T, int64_t V,
