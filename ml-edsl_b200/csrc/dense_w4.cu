@@ -23,9 +23,8 @@
 // Layout (w4_pack): strips of 64 columns; in a strip, blocks of 64 of K; in a
 // block, four 512-byte pieces of 16 columns, 16 bytes for each lane: the
 // codes of its fragments of four k16 steps, in an order that takes one shift
-// and one and-or for two weights. K inside a block is permuted so that a
-// lane's activations are 16 contiguous bytes. Scales and zeros lie in the
-// order in which the lanes read them.
+// and one and-or for two weights. Scales and zeros lie in the order in which
+// the lanes read them.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <algorithm>
@@ -56,7 +55,7 @@ namespace {
 // its block, and its column within the 16 columns of the piece.
 __host__ __device__ __forceinline__ void code_place(int lane, int j, int nib, int* k, int* n) {
   const int g = lane >> 2, t = lane & 3, r = nib & 3;
-  *k = (j >> 1) * 32 + t * 8 + (j & 1) * 4 + (r >> 1) * 2 + (nib >> 2);
+  *k = j * 16 + t * 2 + (r >> 1) * 8 + (nib >> 2);
   *n = g + (r & 1) * 8;
 }
 
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
     dense_w4_few_kernel(const __grid_constant__ W4Params p) {
   using X = XRow<XT>;
   using Mma = typename X::Mma;
-  using T = typename X::T;
+  using Raw = typename X::Raw;
   constexpr int MT = 4, SUBS = FINE ? 2 : 1, THREADS = kFewWarps * 32;
   extern __shared__ __align__(16) char smem[];
   cg::cluster_group cluster = cg::this_cluster();
@@ -254,9 +253,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
 
   // The activations that are staged first are asked for before the weights.
   int per_row = min(b1 - b0, p.stage_blocks) * 8;  // units of 8 elements
-  const T* xrow = static_cast<const T*>(a.X) + m0 * a.ldx;
-  auto load_x = [&](int s0, int m, int c, T (&e)[8]) {
-    load8(xrow + m * a.ldx, (int64_t)s0 * kBlockK + c * 8, K, p.x_aligned, e);
+  const char* xrow = static_cast<const char*>(a.X) + m0 * a.ldx * X::kBytes;
+  auto load_x = [&](int s0, int m, int c) {
+    return X::load(xrow + m * a.ldx * X::kBytes, (int64_t)s0 * kBlockK + c * 8, K, p.x_aligned);
   };
   auto next_unit = [&](int& m, int& c) {
     while (c >= per_row) {
@@ -264,11 +263,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
       ++m;
     }
   };
-  __align__(16) T first[8];
+  Raw first = {};
   int m = 0, c = tid;
   if (b0 < b1) {
     next_unit(m, c);
-    if (m < mrows) load_x(b0, m, c, first);
+    if (m < mrows) first = load_x(b0, m, c);
   }
 #pragma unroll
   for (int i = 0; i < kDepth; ++i) fetch(i);
@@ -296,19 +295,27 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
       m = 0;
       c = tid;
       next_unit(m, c);
-      if (m < mrows) load_x(s0, m, c, first);
+      if (m < mrows) first = load_x(s0, m, c);
     }
-    auto store_x = [&](int m, int c, const T (&e)[8]) {
+    auto store_x = [&](int m, int c, const Raw& e) {
       uint4 out[X::kParts];
       X::stage(e, out);
+      // Pair t of piece c is word c % 4 of the 16 bytes that lane t of a column
+      // reads for 32 of K.
 #pragma unroll
-      for (int q = 0; q < X::kParts; ++q)
-        *reinterpret_cast<uint4*>(xsm + (m * X::kParts + q) * pitch + c * 16) = out[q];
+      for (int q = 0; q < X::kParts; ++q) {
+        uint32_t* to = reinterpret_cast<uint32_t*>(xsm + (m * X::kParts + q) * pitch +
+                                                   (c >> 2) * 64 + (c & 3) * 4);
+        to[0] = out[q].x;
+        to[4] = out[q].y;
+        to[8] = out[q].z;
+        to[12] = out[q].w;
+      }
     };
     if (m < mrows) store_x(m, c, first);
     while (m < mrows) {  // the others, four loads at a time
       constexpr int U = 4;
-      __align__(16) T e[U][8];
+      Raw e[U];
       int um[U], uc[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
         next_unit(m, c);
         um[u] = m;
         uc[u] = c;
-        if (m < mrows) load_x(s0, m, c, e[u]);
+        if (m < mrows) e[u] = load_x(s0, m, c);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)

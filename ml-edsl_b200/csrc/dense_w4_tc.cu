@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
     dense_w4_tc_kernel(const __grid_constant__ W4Params p, int* status) {
   using X = XRow<XT>;
   using Mma = typename X::Mma;
-  using T = typename X::T;
+  using Raw = typename X::Raw;
   constexpr int PARTS = X::kParts, HALF = NC / 2, SUMS = sum_buffers(NC);
   constexpr bool BF16 = Mma::kMagic == MmaBF16::kMagic;
   constexpr uint32_t kIdesc = idesc_16bit_f32(BF16, kTileN, NC);
@@ -241,49 +241,81 @@ __global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
     while (folded < units && ok) ok = fold(folded++);
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (wid < kWorkers + kStagers) {
-    // ---- activations: 16-byte pieces of 8 elements, 8 pieces a row and block
+    // ---- activations: pieces of 8 elements, 8 of a row and block; 16 bytes
+    // of the column's 128 in shared memory, swizzled as the tensor core reads
+    // them
     constexpr int PER = (NC / PARTS * 8 + kStagers * 32 - 1) / (kStagers * 32);
     const int st = tid - kWorkers * 32;
-    const int c = st & 7;
-    const T* xrow = static_cast<const T*>(a.X) + m0 * a.ldx;
-    __align__(16) T next[PER][8];
-    auto load = [&](int i) {
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        const int m = (st >> 3) + u * (kStagers * 4);
-        if (m < mrows && i < nb)
-          load8(xrow + m * a.ldx, (int64_t)(b0 + i) * kBlockK + c * 8, K, p.x_aligned, next[u]);
-      }
+    const int c = st & 7, row0 = st >> 3, rows_step = kStagers * 4;
+    const char* x = static_cast<const char*>(a.X) + m0 * a.ldx * X::kBytes;
+    auto place = [&](int stage, int col) {
+      return xring + stage * NC * 128 + col * 128 + ((c ^ (col & 7)) << 4);
     };
-    load(0);
-    for (int i = 0; i < nb; ++i) {
-      const int stage = i % kStages;
-      if (i >= kStages && !mbar_wait(&bar->empty[stage], (i / kStages - 1) & 1, status,
-                                     kDevTimeoutEmpty, abort_flag))
-        break;
-      char* tile = xring + stage * NC * 128;
-#pragma unroll
-      for (int u = 0; u < PER; ++u) {
-        const int m = (st >> 3) + u * (kStagers * 4);
-        if (m >= mrows) continue;
-        uint4 out[PARTS];
-        X::stage(next[u], out);
-#pragma unroll
-        for (int q = 0; q < PARTS; ++q) {
-          const int col = m * PARTS + q;
-          const uint32_t w[4] = {out[q].x, out[q].y, out[q].z, out[q].w};
-          // the k order of the packed codes: pair j of a piece goes to chunk
-          // 4 * (c / 4) + j, word c % 4, of the column's 128 swizzled bytes
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint32_t*>(tile + col * 128 + ((((c >> 2) * 4 + j) ^ (col & 7)) << 4) +
-                                         (c & 3) * 4) = w[j];
-        }
-      }
+    auto room = [&](int i) {
+      return i < kStages || mbar_wait(&bar->empty[i % kStages], (i / kStages - 1) & 1, status,
+                                      kDevTimeoutEmpty, abort_flag);
+    };
+    auto post = [&](int i) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->full[stage]);
-      load(i + 1);
+      if (lane == 0) mbar_arrive(&bar->full[i % kStages]);
+    };
+    if (X::kBytes == 2 && p.x_aligned) {
+      // 16-bit rows are copied as they are, kAhead blocks ahead
+      constexpr int kAhead = 2;
+      for (int i = 0; i < nb + kAhead; ++i) {
+        if (i < nb) {
+          if (!room(i)) break;
+          const int k = (b0 + i) * kBlockK + c * 8;
+          const int bytes = max(0, min(16, (K - k) * 2));
+#pragma unroll
+          for (int u = 0; u < PER; ++u) {
+            const int m = row0 + u * rows_step;
+            if (m < mrows)
+              cp_async16_fill(place(i % kStages, m), x + ((int64_t)m * a.ldx + (bytes ? k : 0)) * 2,
+                              bytes);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (i >= kAhead) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+          post(i - kAhead);
+        }
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+      // others pass through registers, asked for one block ahead
+      Raw next[PER];
+      auto load = [&](int i) {
+        if (i >= nb) return;
+        const int64_t k = (int64_t)(b0 + i) * kBlockK + c * 8;
+        if (p.x_aligned && (b0 + i + 1) * kBlockK <= K) {
+#pragma unroll
+          for (int u = 0; u < PER; ++u)  // rows past the last: the last again
+            next[u] = X::load_whole(x + min(row0 + u * rows_step, mrows - 1) * a.ldx * X::kBytes, k);
+        } else {
+#pragma unroll
+          for (int u = 0; u < PER; ++u)
+            next[u] = X::load(x + min(row0 + u * rows_step, mrows - 1) * a.ldx * X::kBytes, k, K,
+                              false);
+        }
+      };
+      load(0);
+      for (int i = 0; i < nb; ++i) {
+        if (!room(i)) break;
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          const int m = row0 + u * rows_step;
+          if (m >= mrows) continue;
+          uint4 out[PARTS];
+          X::stage(next[u], out);
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q)
+            *reinterpret_cast<uint4*>(place(i % kStages, m * PARTS + q)) = out[q];
+        }
+        load(i + 1);
+        post(i);
+      }
     }
   } else if (lane == 0) {
     // ---- products

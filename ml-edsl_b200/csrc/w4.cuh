@@ -75,21 +75,31 @@ struct MmaF16 {
   }
 };
 
-// How rows of X become operand columns: kParts columns for a row. stage()
-// takes 8 consecutive elements and gives 16 bytes for each column.
+// How rows of X become operand columns: kParts columns for a row. load() takes
+// 8 consecutive elements of a row from column k on, 0 from `end` on, into
+// registers (load_whole(): aligned ones, all there); stage() makes 16 bytes for each column of them.
 template <int XT>
 struct XRow;
 template <>
 struct XRow<kBF16> {
   using Mma = MmaBF16;
-  using T = uint16_t;
-  static constexpr int kParts = 1;
-  static __device__ __forceinline__ void stage(const T (&e)[8], uint4 (&out)[1]) {
+  using Raw = uint4;
+  static constexpr int kParts = 1, kBytes = 2;
+  static __device__ __forceinline__ Raw load_whole(const char* row, int64_t k) {
+    return __ldg(reinterpret_cast<const uint4*>(row + k * 2));
+  }
+  static __device__ __forceinline__ Raw load(const char* row, int64_t k, int64_t end,
+                                             bool aligned) {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(row) + k;
+    if (aligned && k + 8 <= end) return load_whole(row, k);
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
-    out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 4; ++i)
+      w[i] = (k + 2 * i < end ? __ldg(e + 2 * i) : 0u) |
+             (k + 2 * i + 1 < end ? (uint32_t)__ldg(e + 2 * i + 1) : 0u) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
+  static __device__ __forceinline__ void stage(const Raw& r, uint4 (&out)[1]) { out[0] = r; }
 };
 template <>
 struct XRow<kF16> : XRow<kBF16> {
@@ -98,14 +108,28 @@ struct XRow<kF16> : XRow<kBF16> {
 template <>
 struct XRow<kE4M3> {
   using Mma = MmaF16;
-  using T = uint8_t;
-  static constexpr int kParts = 1;
-  static __device__ __forceinline__ void stage(const T (&e)[8], uint4 (&out)[1]) {
+  using Raw = uint2;
+  static constexpr int kParts = 1, kBytes = 1;
+  static __device__ __forceinline__ Raw load_whole(const char* row, int64_t k) {
+    return __ldg(reinterpret_cast<const uint2*>(row + k));
+  }
+  static __device__ __forceinline__ Raw load(const char* row, int64_t k, int64_t end,
+                                             bool aligned) {
+    const uint8_t* e = reinterpret_cast<const uint8_t*>(row) + k;
+    if (aligned && k + 8 <= end) return load_whole(row, k);
+    uint32_t w[2] = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < end) w[i >> 2] |= (uint32_t)__ldg(e + i) << (8 * (i & 3));
+    return make_uint2(w[0], w[1]);
+  }
+  static __device__ __forceinline__ void stage(const Raw& r, uint4 (&out)[1]) {
+    const uint32_t in[2] = {r.x, r.y};
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-          (__nv_fp8x2_storage_t)(e[2 * i] | (uint16_t)e[2 * i + 1] << 8), __NV_E4M3);
+          (__nv_fp8x2_storage_t)(in[i >> 1] >> (16 * (i & 1)) & 0xffffu), __NV_E4M3);
       w[i] = h.x | (uint32_t)h.y << 16;
     }
     out[0] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -114,49 +138,50 @@ struct XRow<kE4M3> {
 template <>
 struct XRow<kF32> {
   using Mma = MmaBF16;
-  using T = uint32_t;
-  static constexpr int kParts = 3;
+  struct Raw {
+    uint4 a, b;
+  };
+  static constexpr int kParts = 3, kBytes = 4;
+  static __device__ __forceinline__ Raw load_whole(const char* row, int64_t k) {
+    const uint4* e = reinterpret_cast<const uint4*>(row + k * 4);
+    return {__ldg(e), __ldg(e + 1)};
+  }
+  static __device__ __forceinline__ Raw load(const char* row, int64_t k, int64_t end,
+                                             bool aligned) {
+    const uint32_t* e = reinterpret_cast<const uint32_t*>(row) + k;
+    if (aligned && k + 8 <= end) return load_whole(row, k);
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = k + i < end ? __ldg(e + i) : 0u;
+    return {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
+  }
   // x = hi + mid + lo, each the leading 8 bits of what is left (cut, so that
   // no part rounds up out of range). Infinities and NaN travel in hi.
-  static __device__ __forceinline__ void stage(const T (&e)[8], uint4 (&out)[3]) {
-    uint32_t p[3][8];
+  static __device__ __forceinline__ void stage(const Raw& r, uint4 (&out)[3]) {
+    const uint32_t e[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    uint32_t w[3][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool finite = (e[i] & 0x7f800000u) != 0x7f800000u;
-      const bool nan = !finite && (e[i] & 0x007fffffu);
-      p[0][i] = nan ? 0x7fc0u : e[i] >> 16;
-      const float r = __uint_as_float(e[i]) - __uint_as_float(e[i] & 0xffff0000u);
-      const uint32_t rb = __float_as_uint(r) & 0xffff0000u;
-      p[1][i] = finite ? rb >> 16 : 0u;
-      p[2][i] = finite ? __float_as_uint(r - __uint_as_float(rb)) >> 16 : 0u;
+    for (int i = 0; i < 4; ++i) {
+      uint32_t p[3][2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t x = e[2 * i + h];
+        const bool finite = (x & 0x7f800000u) != 0x7f800000u;
+        const bool nan = !finite && (x & 0x007fffffu);
+        p[0][h] = nan ? 0x7fc00000u : x;
+        const float rest = __uint_as_float(x) - __uint_as_float(x & 0xffff0000u);
+        const uint32_t mid = __float_as_uint(rest);
+        const uint32_t lo = __float_as_uint(rest - __uint_as_float(mid & 0xffff0000u));
+        p[1][h] = finite ? mid : 0u;
+        p[2][h] = finite ? lo : 0u;
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q) w[q][i] = __byte_perm(p[q][0], p[q][1], 0x7632);  // upper halves
     }
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
-      uint32_t w[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = p[q][2 * i] | p[q][2 * i + 1] << 16;
-      out[q] = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+    for (int q = 0; q < 3; ++q) out[q] = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
   }
 };
-
-// Eight elements of a row of X from column k on, 0 from `end` on.
-template <class T>
-__device__ __forceinline__ void load8(const T* row, int64_t k, int64_t end, bool aligned,
-                                      T (&e)[8]) {
-  if (aligned && k + 8 <= end) {
-    if constexpr (sizeof(T) == 1) {
-      *reinterpret_cast<uint2*>(e) = __ldg(reinterpret_cast<const uint2*>(row + k));
-    } else {
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        reinterpret_cast<uint4*>(e)[i] = __ldg(reinterpret_cast<const uint4*>(row + k) + i);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = k + i < end ? __ldg(row + k + i) : T(0);
-  }
-}
 
 __device__ __forceinline__ float activate(float x, int act, float alpha) {
   if (act == kActRelu) return (x > 0.0f || x != x) ? x : 0.0f;
@@ -189,6 +214,13 @@ struct W4Params {
 __device__ __forceinline__ void cp_async16(void* smem, const void* global) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(smem)),
                "l"(global)
+               : "memory");
+}
+
+// `bytes` (0 to 16) of them, zeros for the rest.
+__device__ __forceinline__ void cp_async16_fill(void* smem, const void* global, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem)), "l"(global),
+               "r"(bytes)
                : "memory");
 }
 
