@@ -547,7 +547,7 @@ template <int XT>
 int dispatch(const W4Params& p, int* status, cudaStream_t st) {
   const bool fine = p.a.w.group == 32 || p.a.x_group == 32;
   const int64_t cols = p.a.M * XRow<XT>::kParts;
-  static const int most = getenv("W4MOST") ? atoi(getenv("W4MOST")) : 8;
+  static const int most = getenv("W4MOST") ? atoi(getenv("W4MOST")) : 16;
   if (cols > most) return dense_w4_tc(p, status, st);
   if (cols <= 8) return fine ? launch_few<XT, 1, true>(p, st) : launch_few<XT, 1, false>(p, st);
   return fine ? launch_few<XT, 2, true>(p, st) : launch_few<XT, 2, false>(p, st);

@@ -8,17 +8,18 @@
 // pair as in dense_w4.cu) and are stored to TMEM, never to shared memory.
 //
 // A CTA has 128 columns of W, up to NC operand columns and its part of K (the
-// CTAs of a cluster share K), and 13 warps:
-//   0-7   two sets of four, a set for every other block of 64 of K: codes
-//         (copied ahead by the lanes that use them) to TMEM; then the sums of
-//         a unit of K out of TMEM, times its scale, into registers, each set
-//         half of the columns
-//   8-11  activations, one block ahead in registers, into shared memory
-//   12    issues the products
+// CTAs of a cluster share K), and its warps one task each:
+//   8 warps   codes, copied ahead by the lanes that use them, to TMEM
+//   4 warps   activations, a stage ahead, into shared memory
+//   1 warp    issues the products
+//   4 or 8    sums out of TMEM, times their scales, into registers
 // A unit is what one scale covers, at most 128 of K: products are exact, the
 // tensor core sums 8 k16 steps at most, and the rest is added in f32 as for
-// few rows. Every wait is bounded; one that runs out ends all roles and is
-// reported by b200_stream_sync.
+// few rows. Measured on B200, a product of up to 64 columns takes 47 cycles to
+// issue, a commit 190 and each meeting of two roles about as long, so they
+// meet once for a stage of up to four blocks of K, with one commit for its
+// operands and its sums. Every wait is bounded; one that runs out ends all
+// roles and is reported by b200_stream_sync.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <algorithm>
@@ -33,35 +34,46 @@ namespace b200 {
 namespace {
 
 constexpr int kTileN = 128;
-constexpr int kStages = 4;         // blocks of K between the roles
-constexpr int kWorkers = 8;        // warps that expand codes and fold sums
-constexpr int kStagers = 4;        // warps that bring activations
-constexpr int kThreads = (kWorkers + kStagers + 1) * 32;
-constexpr int kCodeDepth = 4;      // blocks that a lane copies ahead
-constexpr int kTmemA = kStages * 32;  // TMEM columns of the expanded weights
+constexpr int kExpanders = 8;  // warps that expand codes, in two sets
+constexpr int kStagers = 4;    // warps that bring activations
+constexpr int kCodeDepth = 8;  // blocks that a lane copies ahead
+constexpr int kMaxStages = 3;
 
-// TMEM columns: 256 where two CTAs fit an SM.
-__host__ __device__ constexpr int tmem_columns(int NC) { return NC <= 64 ? 256 : 512; }
-__host__ __device__ constexpr int sum_buffers(int NC) {
-  return (tmem_columns(NC) - kTmemA) / NC < 4 ? (tmem_columns(NC) - kTmemA) / NC : 4;
-}
+// A stage: kBlocks blocks of 64 of K and the kUnits sums of NC columns that
+// they take; as many blocks (1, 2 or 4) as let two stages fit TMEM's 512
+// columns.
+template <int NC, int UNIT>
+struct Stage {
+  static constexpr int columns(int blocks) {
+    return 32 * blocks + (64 * blocks > UNIT ? 64 * blocks / UNIT : 1) * NC;
+  }
+  static constexpr int kBlocks = columns(4) <= 256 ? 4 : columns(2) <= 256 ? 2 : 1;
+  static constexpr int kUnits = 64 * kBlocks > UNIT ? 64 * kBlocks / UNIT : 1;
+  static constexpr int kColumns = 32 * kBlocks + kUnits * NC;
+  static constexpr int kCount = 512 / kColumns < kMaxStages ? 512 / kColumns : kMaxStages;
+  static constexpr int kFolders = NC <= 32 ? 4 : 8;  // warps that fold sums
+  static constexpr int kThreads = (kExpanders + kStagers + 1 + kFolders) * 32;
+  static_assert(kCount >= 2, "two stages fit TMEM");
+};
 
 struct Barriers {
-  uint64_t full[kStages];   // codes and activations of a block are in place
-  uint64_t empty[kStages];  // its products are done
-  uint64_t sums[4];         // the sums of a unit are complete
-  uint64_t taken[4];        // and have been read
+  uint64_t full[kMaxStages];   // codes and activations of a stage are in place
+  uint64_t done[kMaxStages];   // its products are done, its sums complete
+  uint64_t taken[kMaxStages];  // its sums have been read
   uint32_t tmem;
   int abort_flag;
 };
 
 template <int XT, int NC, int UNIT>
-__global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
     dense_w4_tc_kernel(const __grid_constant__ W4Params p, int* status) {
   using X = XRow<XT>;
   using Mma = typename X::Mma;
   using Raw = typename X::Raw;
-  constexpr int PARTS = X::kParts, HALF = NC / 2, SUMS = sum_buffers(NC);
+  using S = Stage<NC, UNIT>;
+  constexpr int PARTS = X::kParts, OWN = NC / (S::kFolders / 4), STAGES = S::kCount, SB = S::kBlocks;
+  constexpr int kMmaWarp = kExpanders + kStagers, kFoldWarp = kMmaWarp + 1;
+  constexpr int SUBS = UNIT == 32 ? 2 : 1;  // scales of a block
   constexpr bool BF16 = Mma::kMagic == MmaBF16::kMagic;
   constexpr uint32_t kIdesc = idesc_16bit_f32(BF16, kTileN, NC);
   extern __shared__ __align__(1024) char smem[];
@@ -74,53 +86,56 @@ __global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
   const int64_t m0 = (int64_t)blockIdx.y * p.rows;
   const int mrows = (int)min((int64_t)p.rows, a.M - m0);
   const int K = (int)a.w.K, kblocks = (int)p.kblocks;
-  // blocks of K of this CTA, in whole units
-  constexpr int UB = UNIT / 64 > 0 ? UNIT / 64 : 1;  // blocks of a unit
-  const int groups_of_blocks = (kblocks + UB - 1) / UB;
-  const int b0 = (int)((int64_t)groups_of_blocks * rank >> log_c) * UB;
-  const int b1 = min(kblocks, (int)((int64_t)groups_of_blocks * (rank + 1) >> log_c) * UB);
-  const int nb = b1 - b0;
+  // this CTA's blocks of K, in whole stages (and so whole units)
+  const int all_stages = (kblocks + SB - 1) / SB;
+  const int b0 = (int)((int64_t)all_stages * rank >> log_c) * SB;
+  const int b1 = min(kblocks, (int)((int64_t)all_stages * (rank + 1) >> log_c) * SB);
+  const int nb = max(0, b1 - b0), stages = (nb + SB - 1) / SB;
   const int units = nb > 0 ? (min(K, b1 * kBlockK) - b0 * kBlockK + UNIT - 1) / UNIT : 0;
 
   // shared memory: activations (swizzled tiles of 64 k by NC columns), codes,
   // what the cluster's CTAs send, barriers
   char* xring = smem;
-  char* cring = xring + kStages * NC * 128;
-  float* recv = reinterpret_cast<float*>(cring + kWorkers * kCodeDepth * 1024);
+  char* cring = xring + STAGES * SB * NC * 128;
+  float* recv = reinterpret_cast<float*>(cring + kExpanders * kCodeDepth * 1024);
   Barriers* bar = reinterpret_cast<Barriers*>(reinterpret_cast<char*>(recv) + p.recv_bytes);
   volatile int* abort_flag = &bar->abort_flag;
   if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&bar->full[i], kWorkers / 2 + kStagers);
-      mbar_init(&bar->empty[i], 1);
-    }
-    for (int i = 0; i < SUMS; ++i) {
-      mbar_init(&bar->sums[i], 1);
-      mbar_init(&bar->taken[i], kWorkers);
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&bar->full[i], (SB > 1 ? kExpanders : kExpanders / 2) + kStagers);
+      mbar_init(&bar->done[i], 1);
+      mbar_init(&bar->taken[i], S::kFolders);
     }
     bar->abort_flag = 0;
     fence_barrier_init();
   }
   pdl_wait();
-  if (wid == kWorkers + kStagers) tmem_alloc(&bar->tmem, tmem_columns(NC));
+  if (wid == kMmaWarp) tmem_alloc(&bar->tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   // only now: a kernel that starts early must not take TMEM that a CTA of this
   // one still waits for
   pdl_trigger();
-  const uint32_t tmem = bar->tmem, tmem_sums = tmem + kTmemA;
+  const uint32_t tmem = bar->tmem, tmem_sums = tmem + STAGES * SB * 32;
+  // the products of stage t's predecessor in the ring are done
+  auto reusable = [&](int t) {
+    return t < STAGES || mbar_wait_long(&bar->done[t % STAGES], (t / STAGES - 1) & 1, status,
+                                        kDevTimeoutEmpty, abort_flag);
+  };
 
-  float total[HALF];
+  const int quarter = wid & 3;  // of TMEM's lanes, where a warp has one
+  float total[OWN];             // of a folding warp
 #pragma unroll
-  for (int i = 0; i < HALF; ++i) total[i] = 0.0f;
-  const int quarter = wid & 3, set = wid >> 2;  // of a worker
+  for (int i = 0; i < OWN; ++i) total[i] = 0.0f;
+  const int fold_set = (wid - kFoldWarp) >> 2;
 
-  if (wid < kWorkers) {
-    const int64_t strip = n0 / kStripN + (quarter >> 1);
-    const bool live = strip * kStripN < a.w.N;
-    const int mt0 = (quarter & 1) * 2, g = lane >> 2;
-    // ---- codes: two 16-column pieces of the quarter's 32 columns
+  const int64_t strip = n0 / kStripN + (quarter >> 1);
+  const bool live = strip * kStripN < a.w.N;
+  if (wid < kExpanders) {
+    const int set = wid >> 2, mt0 = (quarter & 1) * 2, g = lane >> 2;
+    // ---- codes: two 16-column pieces of the quarter's 32 columns; the set's
+    // blocks are every other one
     uint4* mine = reinterpret_cast<uint4*>(cring) + wid * (kCodeDepth * 64) + lane;
     const uint4* codes = p.codes + ((strip * kblocks + b0 + set) * 4 + mt0) * 32 + lane;
     int fetched = set;
@@ -136,11 +151,11 @@ __global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < kCodeDepth; ++i) fetch(i);
     const uint8_t* zeros = p.zeros ? p.zeros + strip * p.groups * 64 + g * 8 + mt0 * 2 : nullptr;
-    uint32_t znext[UNIT == 32 ? 2 : 1] = {};
+    uint32_t znext[SUBS] = {};
     auto fetch_zeros = [&](int i) {
       if (!zeros || !live || i >= nb) return;
 #pragma unroll
-      for (int sub = 0; sub < (UNIT == 32 ? 2 : 1); ++sub) {
+      for (int sub = 0; sub < SUBS; ++sub) {
         const int k = (b0 + i) * kBlockK + sub * 32;
         if (sub && k >= K) return;
         znext[sub] =
@@ -148,73 +163,19 @@ __global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
       }
     };
     fetch_zeros(set);
-    // ---- scales: this lane's column of W, for the unit that is folded next
-    const int n = (quarter & 1) * 32 + lane;  // within the strip
-    const int64_t scale_col = strip * p.groups * 64 + column_place(n);
-    auto scale_of_unit = [&](int u) {
-      const int k = b0 * kBlockK + u * UNIT;
-      return live && u < units
-                 ? load_as_f32(p.scales, a.w.s_dtype, scale_col + (int64_t)p.group_of(k) * 64)
-                 : 0.0f;
-    };
-    float scale_next = scale_of_unit(0);
-
-    bool ok = true;
-    int folded = 0, slot = 0;
-    auto fold = [&](int u) {
-      const int buf = u % SUMS;
-      if (!mbar_wait(&bar->sums[buf], (u / SUMS) & 1, status, kDevTimeoutAccum, abort_flag))
-        return false;
-      tc_fence_after();
-      const float scale = scale_next;
-      scale_next = scale_of_unit(u + 1);
-      const uint32_t from = tmem_sums + ((uint32_t)(quarter * 32) << 16) + buf * NC + set * HALF;
-      constexpr int STEP = HALF < 16 ? 8 : 16;
-#pragma unroll
-      for (int c = 0; c < HALF; c += STEP) {
-        uint32_t v[STEP];
-        if constexpr (STEP == 8) tmem_ld_32x32b_x8(from + c, v);
-        else tmem_ld_32x32b_x16(from + c, v);
-        tmem_ld_wait();
-        if (XT == kE4M3 && a.x_group > 0) {
-          const unsigned xg = (unsigned)(b0 * kBlockK + u * UNIT) / (unsigned)a.x_group;
-#pragma unroll
-          for (int i = 0; i < STEP; ++i) {
-            const int m = set * HALF + c + i;
-            const float xs = m < mrows ? __ldg(a.x_scales + (m0 + m) * a.ldxs + xg) : 0.0f;
-            total[c + i] = fmaf(__uint_as_float(v[i]) * xs, scale, total[c + i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < STEP; ++i)
-            total[c + i] = fmaf(__uint_as_float(v[i]), scale, total[c + i]);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->taken[buf]);
-      return true;
-    };
-    for (int i = set; i < nb && ok; i += 2) {
-      const int stage = i % kStages;
+    int slot = 0;
+    // block i (of the set's) to the columns of TMEM from `to` on
+    auto expand = [&](int i, uint32_t to) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kCodeDepth - 1) : "memory");
-      uint4 w[2];
-      w[0] = mine[slot * 64];
-      w[1] = mine[slot * 64 + 32];
-      uint32_t z[UNIT == 32 ? 2 : 1][4];
+      const uint4 w[2] = {mine[slot * 64], mine[slot * 64 + 32]};
+      uint32_t z[SUBS][4];
 #pragma unroll
-      for (int sub = 0; sub < (UNIT == 32 ? 2 : 1); ++sub)
+      for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           z[sub][q] = zeros ? __byte_perm(znext[sub], Mma::kMagic, 0x5050 | q * 0x0101)
                             : 0x00080008u | Mma::kMagic;
       fetch_zeros(i + 2);
-      if (i >= kStages && !mbar_wait(&bar->empty[stage], (i / kStages - 1) & 1, status,
-                                     kDevTimeoutEmpty, abort_flag)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const uint32_t words[4] = {w[q].x, w[q].y, w[q].z, w[q].w};
@@ -224,65 +185,71 @@ __global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             f[4 * j + r] = Mma::sub(and_or(words[j] >> (4 * r), 0x000f000fu, Mma::kMagic),
-                                    z[UNIT == 32 ? j >> 1 : 0][2 * q + (r & 1)]);
-        tmem_st_16x128b_x8(tmem + ((uint32_t)(quarter * 32 + q * 16) << 16) + stage * 32, f);
+                                    z[SUBS == 2 ? j >> 1 : 0][2 * q + (r & 1)]);
+        tmem_st_16x128b_x8(to + ((uint32_t)(quarter * 32 + q * 16) << 16), f);
+      }
+      fetch(slot);  // the slot's codes have been used
+      slot = (slot + 1) % kCodeDepth;
+    };
+
+    for (int t = 0; t < stages; ++t) {
+      if (SB == 1 && (t & 1) != set) continue;
+      if (!reusable(t)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int b = 0; b < (SB + 1) / 2; ++b) {
+        const int in_stage = SB > 1 ? 2 * b + set : 0, i = t * SB + in_stage;
+        if (i < nb) expand(i, tmem + (t % STAGES * SB + in_stage) * 32);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->full[stage]);
-      fetch(slot);  // the slot's codes have been used
-      slot = (slot + 1) % kCodeDepth;
-      // fold what is complete two blocks behind: the products of blocks that
-      // both sets have expanded
-      const int upto = min(units, UNIT == 32 ? 2 * (i - 1) : (i - 1) / UB);
-      while (folded < upto && ok) ok = fold(folded++);
+      if (lane == 0) mbar_arrive(&bar->full[t % STAGES]);
     }
-    while (folded < units && ok) ok = fold(folded++);
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (wid < kWorkers + kStagers) {
+  } else if (wid < kMmaWarp) {
     // ---- activations: pieces of 8 elements, 8 of a row and block; 16 bytes
     // of the column's 128 in shared memory, swizzled as the tensor core reads
     // them
     constexpr int PER = (NC / PARTS * 8 + kStagers * 32 - 1) / (kStagers * 32);
-    const int st = tid - kWorkers * 32;
+    const int st = tid - kExpanders * 32;
     const int c = st & 7, row0 = st >> 3, rows_step = kStagers * 4;
     const char* x = static_cast<const char*>(a.X) + m0 * a.ldx * X::kBytes;
-    auto place = [&](int stage, int col) {
-      return xring + stage * NC * 128 + col * 128 + ((c ^ (col & 7)) << 4);
+    // column `col` of block i
+    auto place = [&](int i, int col) {
+      return xring + (i / SB % STAGES * SB + i % SB) * (NC * 128) + col * 128 +
+             ((c ^ (col & 7)) << 4);
     };
-    auto room = [&](int i) {
-      return i < kStages || mbar_wait(&bar->empty[i % kStages], (i / kStages - 1) & 1, status,
-                                      kDevTimeoutEmpty, abort_flag);
-    };
-    auto post = [&](int i) {
+    auto post = [&](int t) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->full[i % kStages]);
+      if (lane == 0) mbar_arrive(&bar->full[t % STAGES]);
     };
     if (X::kBytes == 2 && p.x_aligned) {
-      // 16-bit rows are copied as they are, kAhead blocks ahead
-      constexpr int kAhead = 2;
-      for (int i = 0; i < nb + kAhead; ++i) {
-        if (i < nb) {
-          if (!room(i)) break;
-          const int k = (b0 + i) * kBlockK + c * 8;
-          const int bytes = max(0, min(16, (K - k) * 2));
+      // 16-bit rows are copied as they are
+      const int k0 = b0 * kBlockK + c * 8;
+      const int64_t step = (int64_t)rows_step * a.ldx * 2;
+      const char* from = x + ((int64_t)row0 * a.ldx + k0) * 2;
+      int left = (K - k0) * 2;      // bytes of the row from here on
+      int64_t at_start = x - from;  // a valid address where nothing is read
+      for (int t = 0; t < stages; ++t) {
+        if (!reusable(t)) break;
 #pragma unroll
-          for (int u = 0; u < PER; ++u) {
-            const int m = row0 + u * rows_step;
-            if (m < mrows)
-              cp_async16_fill(place(i % kStages, m), x + ((int64_t)m * a.ldx + (bytes ? k : 0)) * 2,
+        for (int sb = 0; sb < SB; ++sb) {
+          const int bytes = max(0, min(16, left));
+          char* to = place(t * SB + sb, row0);  // rows_step is a multiple of the swizzle's 8
+#pragma unroll
+          for (int u = 0; u < PER; ++u)
+            if (row0 + u * rows_step < mrows)
+              cp_async16_fill(to + u * (rows_step * 128), from + (bytes ? u * step : at_start),
                               bytes);
-          }
+          from += kBlockK * 2;
+          at_start -= kBlockK * 2;
+          left -= kBlockK * 2;
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        if (i >= kAhead) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
-          post(i - kAhead);
-        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        post(t);
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
       // others pass through registers, asked for one block ahead
       Raw next[PER];
@@ -301,114 +268,201 @@ __global__ void __launch_bounds__(kThreads, NC <= 64 ? 2 : 1)
         }
       };
       load(0);
-      for (int i = 0; i < nb; ++i) {
-        if (!room(i)) break;
+      for (int t = 0; t < stages; ++t) {
+        if (!reusable(t)) break;
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-          const int m = row0 + u * rows_step;
-          if (m >= mrows) continue;
-          uint4 out[PARTS];
-          X::stage(next[u], out);
+        for (int sb = 0; sb < SB; ++sb) {
+          const int i = t * SB + sb;
+          if (i < nb) {
 #pragma unroll
-          for (int q = 0; q < PARTS; ++q)
-            *reinterpret_cast<uint4*>(place(i % kStages, m * PARTS + q)) = out[q];
+            for (int u = 0; u < PER; ++u) {
+              const int m = row0 + u * rows_step;
+              if (m >= mrows) continue;
+              uint4 out[PARTS];
+              X::stage(next[u], out);
+#pragma unroll
+              for (int q = 0; q < PARTS; ++q)
+                *reinterpret_cast<uint4*>(place(i, m * PARTS + q)) = out[q];
+            }
+            load(i + 1);
+          }
         }
-        load(i + 1);
-        post(i);
+        post(t);
       }
     }
-  } else if (lane == 0) {
+  } else if (wid == kMmaWarp) {
     // ---- products
-    bool ok = true;
-    int u = 0;
-    for (int i = 0; i < nb && ok; ++i) {
-      const int stage = i % kStages;
-      if (!mbar_wait(&bar->full[stage], (i / kStages) & 1, status, kDevTimeoutFull,
-                     abort_flag)) {
-        ok = false;
+    for (int t = 0; lane == 0 && t < stages; ++t) {
+      const int s = t % STAGES;
+      if (!mbar_wait_long(&bar->full[s], (t / STAGES) & 1, status, kDevTimeoutFull, abort_flag) ||
+          (t >= STAGES && !mbar_wait_long(&bar->taken[s], (t / STAGES - 1) & 1, status,
+                                          kDevTimeoutAccum, abort_flag)))
         break;
-      }
       tc_fence_after();
-      const uint64_t bdesc = umma_desc_k<2, 1024>(smem_u32(xring + stage * NC * 128));
-      const uint32_t at = tmem + stage * 32;
-      constexpr int SUBS = UNIT == 32 ? 2 : 1, STEPS = 4 / SUBS;
+      const uint64_t bdesc = umma_desc_k<2, 1024>(smem_u32(xring + s * SB * NC * 128));
+      const uint32_t from = tmem + s * SB * 32, to = tmem_sums + s * S::kUnits * NC;
 #pragma unroll
-      for (int sub = 0; sub < SUBS; ++sub) {
-        if (u >= units) break;  // the second half of K's last block
-        const int buf = u % SUMS;
-        const bool first = UNIT < 128 || i % UB == 0;
-        if (first && u >= SUMS &&
-            !mbar_wait(&bar->taken[buf], (u / SUMS - 1) & 1, status, kDevTimeoutAccum,
-                       abort_flag)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+      for (int k = 0; k < SB * 4; ++k) {  // k16 steps
+        constexpr int PER_UNIT = UNIT / 16;
+        const int unit = k / PER_UNIT;
+        if (t * SB + k / 4 >= nb || t * S::kUnits + unit >= units) break;
+        umma_f16_ts(to + unit * NC, from + k * 8, bdesc + (k / 4) * (NC * 8) + (k % 4) * 2, kIdesc,
+                    k % PER_UNIT != 0);
+      }
+      umma_commit(&bar->done[s]);
+    }
+  } else {
+    // ---- sums: this lane's column of W, OWN operand columns of it
+    const int n = (quarter & 1) * 32 + lane;  // within the strip
+    const int64_t scale_col = strip * p.groups * 64 + column_place(n);
+    auto scale_of_unit = [&](int u) {
+      const int k = b0 * kBlockK + u * UNIT;
+      return live && u < units
+                 ? load_as_f32(p.scales, a.w.s_dtype, scale_col + (int64_t)p.group_of(k) * 64)
+                 : 0.0f;
+    };
+    float next[S::kUnits];
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
-          const int step = sub * STEPS + k;
-          umma_f16_ts(tmem_sums + buf * NC, at + step * 8, bdesc + step * 2, kIdesc,
-                      !(first && k == 0));
-        }
-        if (UNIT < 128 || i % UB == UB - 1 || i == nb - 1) {
-          umma_commit(&bar->sums[buf]);
-          ++u;
+    for (int j = 0; j < S::kUnits; ++j) next[j] = scale_of_unit(j);
+    for (int t = 0; t < stages; ++t) {
+      const int s = t % STAGES;
+      float scale[S::kUnits];
+#pragma unroll
+      for (int j = 0; j < S::kUnits; ++j) {
+        scale[j] = next[j];
+        next[j] = scale_of_unit((t + 1) * S::kUnits + j);
+      }
+      if (!mbar_wait_long(&bar->done[s], (t / STAGES) & 1, status, kDevTimeoutAccum, abort_flag))
+        break;
+      tc_fence_after();
+      const uint32_t at =
+          tmem_sums + ((uint32_t)(quarter * 32) << 16) + s * S::kUnits * NC + fold_set * OWN;
+#pragma unroll
+      for (int j = 0; j < S::kUnits; ++j) {
+        const int u = t * S::kUnits + j;
+        if (u >= units) break;
+        constexpr int STEP = OWN < 32 ? OWN : OWN == 32 ? 32 : 16;
+#pragma unroll
+        for (int c = 0; c < OWN; c += STEP) {
+          uint32_t v[STEP];
+          if constexpr (STEP == 16) tmem_ld_32x32b_x16(at + j * NC + c, v);
+          else tmem_ld_32x32b_x32(at + j * NC + c, v);
+          tmem_ld_wait();
+          if (XT == kE4M3 && a.x_group > 0) {
+            const unsigned xg = (unsigned)(b0 * kBlockK + u * UNIT) / (unsigned)a.x_group;
+#pragma unroll
+            for (int i = 0; i < STEP; ++i) {
+              const int m = fold_set * OWN + c + i;
+              const float xs = m < mrows ? __ldg(a.x_scales + (m0 + m) * a.ldxs + xg) : 0.0f;
+              total[c + i] = fmaf(__uint_as_float(v[i]) * xs, scale[j], total[c + i]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < STEP; ++i)
+              total[c + i] = fmaf(__uint_as_float(v[i]), scale[j], total[c + i]);
+          }
         }
       }
-      umma_commit(&bar->empty[stage]);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar->taken[s]);
     }
-    // the last arrival is in before shared memory goes
-    if (ok && nb > 0)
-      mbar_wait(&bar->empty[(nb - 1) % kStages], ((nb - 1) / kStages) & 1, status,
-                kDevTimeoutEmpty, abort_flag);
   }
 
   // ---- the CTAs' parts of K: each 32 outputs of a row belong to one CTA of
   // the cluster, in turn
-  const int outs = mrows * kTileN;
-  const int slots = ((mrows * 4 + C - 1) >> log_c) * 32;
+  __syncwarp();
+  const int chunks = mrows * 4;
+  const int slots = ((chunks + C - 1) >> log_c) * 32;
   if (C > 1) cluster.barrier_wait();  // every CTA of the cluster runs
-  if (wid < kWorkers) {
+  if (wid >= kFoldWarp) {
+    float* mine = recv + rank * PARTS * slots + lane;
+    float* to[2];  // for even and odd rows
 #pragma unroll
-    for (int c = 0; c < HALF; ++c) {
-      const int col = set * HALF + c, m = col / PARTS, q = col - m * PARTS;
-      if (m >= mrows) break;
-      const int chunk = m * 4 + quarter;
-      float* dst = recv + (rank * PARTS + q) * slots + (chunk >> log_c) * 32 + lane;
-      *(C > 1 ? cluster.map_shared_rank(dst, chunk & (C - 1)) : dst) = total[c];
+    for (int o = 0; o < 2; ++o)
+      to[o] = C > 1 ? cluster.map_shared_rank(mine, (o * 4 + quarter) & (C - 1)) : mine;
+#pragma unroll
+    for (int c = 0; c < OWN; ++c) {
+      const int col = fold_set * OWN + c, m = col / PARTS, q = col - m * PARTS;
+      if (m < mrows) {
+        const int at = q * slots + ((m * 4 + quarter) >> log_c) * 32;
+        (m & 1 ? to[1] : to[0])[at] = total[c];
+      }
     }
   }
   tc_fence_before();
   if (C > 1) cluster.sync();
   else __syncthreads();
   tc_fence_after();
-  if (wid == kWorkers + kStagers) tmem_dealloc(tmem, tmem_columns(NC));
-  for (int u = tid; u < slots; u += kThreads) {
-    const int o = ((u >> 5 << log_c) + rank) * 32 + (u & 31), m = o >> 7, n = o & 127;
-    if (o >= outs || n0 + n >= a.w.N) continue;
-    float part[PARTS];
+  if (wid == kMmaWarp) tmem_dealloc(tmem, 512);
+  // four outputs a thread
+  const int64_t y_bytes = a.y_dtype == kF32 ? 4 : 2;
+  const bool whole = reinterpret_cast<uintptr_t>(a.Y) % (4 * y_bytes) == 0 && a.ldy % 4 == 0;
+  for (int u = tid * 4; u < slots; u += S::kThreads * 4) {
+    const int chunk = (u >> 5 << log_c) + rank, m = chunk >> 2;
+    const int64_t n = n0 + (chunk & 3) * 32 + (u & 31);
+    if (chunk >= chunks || n >= a.w.N) continue;
+    float4 part[PARTS];
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) part[q] = recv[q * slots + u];
+    for (int q = 0; q < PARTS; ++q) part[q] = *reinterpret_cast<const float4*>(recv + q * slots + u);
     for (int r = 1; r < C; ++r)
 #pragma unroll
-      for (int q = 0; q < PARTS; ++q) part[q] += recv[(r * PARTS + q) * slots + u];
-    float y = part[PARTS - 1];  // the smallest part first
+      for (int q = 0; q < PARTS; ++q) {
+        const float4 v = *reinterpret_cast<const float4*>(recv + (r * PARTS + q) * slots + u);
+        part[q].x += v.x;
+        part[q].y += v.y;
+        part[q].z += v.z;
+        part[q].w += v.w;
+      }
+    float y[4] = {part[PARTS - 1].x, part[PARTS - 1].y, part[PARTS - 1].z, part[PARTS - 1].w};
 #pragma unroll
-    for (int q = PARTS - 2; q >= 0; --q) y += part[q];
-    if (a.x_scales && a.x_group == 0) y *= __ldg(a.x_scales + (m0 + m) * a.ldxs);
-    if (a.b) y += load_as_f32(a.b, a.b_dtype, n0 + n);
-    y = activate(y, a.act, a.alpha);
-    const int64_t at = (m0 + m) * a.ldy + n0 + n;
-    if (a.y_dtype == kF32) static_cast<float*>(a.Y)[at] = y;
-    else if (a.y_dtype == kBF16) static_cast<bf16*>(a.Y)[at] = __float2bfloat16_rn(y);
-    else static_cast<f16*>(a.Y)[at] = __float2half_rn(y);
+    for (int q = PARTS - 2; q >= 0; --q) {  // the smallest part first
+      y[0] += part[q].x;
+      y[1] += part[q].y;
+      y[2] += part[q].z;
+      y[3] += part[q].w;
+    }
+    const float xs = a.x_scales && a.x_group == 0 ? __ldg(a.x_scales + (m0 + m) * a.ldxs) : 1.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (a.x_scales && a.x_group == 0) y[i] *= xs;
+      if (a.b && n + i < a.w.N) y[i] += load_as_f32(a.b, a.b_dtype, n + i);
+      y[i] = activate(y[i], a.act, a.alpha);
+    }
+    char* at = static_cast<char*>(a.Y) + ((m0 + m) * a.ldy + n) * y_bytes;
+    if (a.y_dtype == kF32) {
+      if (whole && n + 4 <= a.w.N) {
+        *reinterpret_cast<float4*>(at) = make_float4(y[0], y[1], y[2], y[3]);
+      } else {
+        for (int i = 0; i < 4 && n + i < a.w.N; ++i) reinterpret_cast<float*>(at)[i] = y[i];
+      }
+      continue;
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (a.y_dtype == kBF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    if (whole && n + 4 <= a.w.N) {
+      *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+    } else {
+      for (int i = 0; i < 4 && n + i < a.w.N; ++i)
+        reinterpret_cast<uint16_t*>(at)[i] = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    }
   }
 }
 
 template <int XT, int NC, int UNIT>
 int launch(W4Params p, int* status, cudaStream_t st) {
   auto kernel = dense_w4_tc_kernel<XT, NC, UNIT>;
-  constexpr int PARTS = XRow<XT>::kParts, PER_SM = NC <= 64 ? 2 : 1;
+  using S = Stage<NC, UNIT>;
+  constexpr int PARTS = XRow<XT>::kParts, PER_SM = 1;
   p.rows = NC / PARTS;
   const int64_t tiles = (p.a.w.N + kTileN - 1) / kTileN;
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
@@ -432,14 +486,14 @@ int launch(W4Params p, int* status, cudaStream_t st) {
   p.log_cluster = best;
   const int rows = (int)std::min<int64_t>(p.rows, p.a.M);
   p.recv_bytes = C * PARTS * ((rows * 4 + C - 1) / C * 32) * 4;
-  const int smem = kStages * NC * 128 + kWorkers * kCodeDepth * 1024 + p.recv_bytes +
+  const int smem = S::kCount * S::kBlocks * NC * 128 + kExpanders * kCodeDepth * 1024 + p.recv_bytes +
                    (int)sizeof(Barriers);
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
   if (e0 != cudaSuccess) return launch_result(e0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)chunks);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2];
@@ -462,7 +516,8 @@ int by_columns(const W4Params& p, int* status, cudaStream_t st) {
   if (cols <= 16) return launch<XT, 16, UNIT>(p, status, st);
   if (cols <= 32) return launch<XT, 32, UNIT>(p, status, st);
   if (cols <= 64) return launch<XT, 64, UNIT>(p, status, st);
-  return launch<XT, 128, UNIT>(p, status, st);
+  // 64 at a time where the sums of 128 do not fit TMEM twice
+  return launch<XT, UNIT == 32 ? 64 : 128, UNIT>(p, status, st);
 }
 
 template <int XT>

@@ -89,6 +89,33 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   return mbar_wait_for(bar, parity, status, code, abort_flag, B200_WAIT_NS);
 }
 
+// mbar_wait for kernels with many waiting warps: each try may suspend the warp
+// for up to 20 us, so that waiting costs next to no issue slots.
+__device__ __forceinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, int* status,
+                                               int code, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  uint64_t start = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    const uint64_t now = globaltimer();
+    if (start == 0) start = now;
+    if (now - start > B200_WAIT_NS) {
+      if (status) atomicCAS(status, 0, code);
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- multicast
 // Stores through an NVSwitch multicast address: one store reaches the same
 // offset in every GPU's memory bound to the multicast object (NVLS).
