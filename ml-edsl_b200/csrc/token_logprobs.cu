@@ -1,28 +1,34 @@
 // Log probabilities of given tokens, entropy and most probable tokens of rows
 // of logits (HBM-bound: every logit is read once).
 //
-// With m = max x, t = x - m, S = sum e^t and D = sum t e^t over a row:
-//   log p(i) = t_i - log S
-//   entropy  = -sum p log p = log S - D / S   (two terms of one sign)
-// Each thread keeps m, S and D of its own logits and rescales them when m
-// grows (D of m' = m + d: e^-d (D - d S)); threads, warps and CTAs are joined
-// the same way, in a fixed order.
+// In powers of two, L = log2 e, with a shift c near m L for the row's maximum m:
+//   t = x L - c (one fma),  S = sum 2^t,  D = sum t 2^t
+//   log p(i) = x_i - m + (m L - c) ln 2 - ln 2 log2 S
+//   entropy  = ln 2 (log2 S - D / S)   (two terms of one sign)
+// The shift is m L rounded to f32: what the rounding leaves is the bracket
+// above, so that t is as exact for logits near 1e4 as near 0. Each thread
+// keeps m, S and D of its own logits and rescales them when m grows (for
+// m' > m, d = c - c': S' = 2^d S, D' = 2^d (D + d S)); threads, warps and CTAs
+// are joined the same way, in a fixed order. Five instructions and one
+// exponential a logit: of bf16 logits an SM has 11.6 a clock to take at the
+// measured bandwidth, of exponentials it has 16.
 //
-// A row is split over the CTAs of a cluster, which join in the first CTA's
-// shared memory: no scratch in device memory, one launch.
+// A row is split over the CTAs of a cluster, which send what they have to the
+// first one's shared memory: no scratch in device memory, one launch.
 //
 // The `top` most probable tokens need no second pass over the row. The k-th
 // largest of the threads' maxima is a lower bound of the k-th largest logit,
 // and only the k threads at or above it hold logits that can be among the
-// first k: the warps read these threads' logits again (L2) and merge what is
-// above the bound into sorted lists of 32. Order: by logit, then the lowest
-// index; NaN ranks as -inf.
+// first k: these threads' logits are read again (L2), and the few that pass
+// the bound are sorted. Order: by logit, then the lowest index; NaN ranks as
+// -inf.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <cstdint>
 #include "dtype.cuh"
 #include "kernels.h"
+#include "ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -31,27 +37,56 @@ namespace b200 {
 namespace {
 
 constexpr float kLowest = -3.402823466e38f;
+constexpr float kLog2E = 1.44269504f, kLn2 = 0.693147181f;
+// Maxima beyond this make x L leave f32: t is then (x - m) L, two roundings.
+constexpr float kWide = 1e38f;
 constexpr unsigned kFull = 0xffffffffu;
 
+__device__ __forceinline__ float minus_inf() { return __int_as_float(0xff800000); }
+__device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fc00000); }
+// 2^t for t <= 0 or so; 0 below -126.
+__device__ __forceinline__ float exp2_fast(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+
+// The shift c of a maximum m. Rounded by itself wherever it is used: a product
+// contracted into an fma would be another number.
+__device__ __forceinline__ float shift_of(float m) { return __fmul_rn(m, kLog2E); }
+
 struct Soft {
-  float m, s, d;  // max, sum e^(x-m), sum (x-m) e^(x-m)
+  float m, s, d;  // max, sum 2^t, sum t 2^t
 };
 
-// a's sums with the maximum m >= a.m. The difference is cut at -200, where
-// e^d is 0 in f32, so that infinite differences give 0 and not NaN.
+// c - c' of two maxima m <= m', at least -200, where 2^d is 0.
+__device__ __forceinline__ float shift_between(float m, float to) {
+  m = fmaxf(m, kLowest);
+  to = fmaxf(to, kLowest);
+  const bool wide = fabsf(m) > kWide || fabsf(to) > kWide;
+  return fmaxf(wide ? (m - to) * kLog2E : __fsub_rn(shift_of(m), shift_of(to)), -200.0f);
+}
+
+// a's sums with the maximum m >= a.m.
 __device__ __forceinline__ void rescale(Soft& a, float m) {
-  const float d = fmaxf(fmaxf(a.m, kLowest) - fmaxf(m, kLowest), -200.0f);
-  const float f = __expf(d);
+  const float d = shift_between(a.m, m), f = exp2_fast(d);
   a.d = f * fmaf(d, a.s, a.d);
   a.s *= f;
   a.m = m;
 }
 
-__device__ __forceinline__ Soft join(Soft a, Soft b) {
-  const float m = fmaxf(a.m, b.m);
+// The sums of a warp's lanes, in every lane.
+__device__ __forceinline__ Soft warp_join(Soft a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, o));
   rescale(a, m);
-  rescale(b, m);
-  return {m, a.s + b.s, a.d + b.d};
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(kFull, a.s, o);
+    a.d += __shfl_xor_sync(kFull, a.d, o);
+  }
+  return a;
 }
 
 // The order of floats as that of unsigned integers; NaN as -inf, -0 as +0.
@@ -105,180 +140,215 @@ __device__ __forceinline__ uint64_t cta_merge(uint64_t v, uint64_t (*sh)[32]) {
   return v;
 }
 
-template <class T>
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// VEC logits, chunk j of the row, into a thread's sums.
+template <int VEC>
 __device__ __forceinline__ void add_chunk(Soft& a, uint32_t& best, uint32_t j, const float* x) {
-  constexpr int VEC = Chunk<T>::kElems;
   float cm = x[0];
 #pragma unroll
-  for (int i = 1; i < VEC; ++i) cm = fmaxf(cm, x[i]);
-  if (cm > a.m) {
-    rescale(a, cm);
-    best = j;
+  for (int i = 1; i < VEC; ++i) cm = max_nan(cm, x[i]);
+  if (!(cm <= a.m)) {  // a new maximum, or NaN
+    float m = a.m;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) m = fmaxf(m, x[i]);
+    if (m > a.m) {
+      rescale(a, m);
+      best = j;
+    }
+    if (cm != cm || cm == __int_as_float(0x7f800000)) a.s = nan_f32();  // no distribution
   }
   const float m = fmaxf(a.m, kLowest);
+  float t[VEC];
+  if (fabsf(m) <= kWide) {
+    const float c = shift_of(m);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = fmaf(x[i], kLog2E, -c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t[i] = (x[i] - m) * kLog2E;
+  }
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const float t = x[i] - m;
-    const float e = __expf(t);
+    t[i] = fmaxf(t[i], -200.0f);  // 2^-200 is 0: -inf adds 0
+    const float e = exp2_fast(t[i]);
     a.s += e;
-    a.d = fmaf(e, fmaxf(t, -200.0f), a.d);  // e^-200 is 0: -inf adds 0
+    a.d = fmaf(e, t[i], a.d);
   }
 }
 
+constexpr int kMaxCandidates = 256;
+constexpr int kMaxCluster = 8;
+
 // Chunk j of a row: its elements [j * VEC - shift, + VEC), which start on 16
 // bytes; the row's first and last chunk may be cut.
-template <class T>
-__global__ void __launch_bounds__(512)
-    token_logprobs_kernel(const __grid_constant__ TokenLogprobsArgs p) {
-  constexpr int VEC = Chunk<T>::kElems, NT = 512, NW = NT / 32, U = 4;
+template <class T, int NT>
+__global__ void __launch_bounds__(NT)
+    token_logprobs_kernel(const __grid_constant__ TokenLogprobsArgs p, int log_c) {
+  constexpr int VEC = Chunk<T>::kElems, NW = NT / 32, U = 4;
   __shared__ Soft sh_soft[NW];
   __shared__ uint64_t sh_keys[NW][32];
+  __shared__ uint64_t sh_candidates[kMaxCandidates];
   __shared__ int sh_flagged[kMaxTop];
-  __shared__ int sh_count;
+  __shared__ int sh_count, sh_found;
   __shared__ uint64_t sh_bound;
+  // what the cluster's CTAs send to the first one
+  __shared__ Soft sh_row[kMaxCluster];
+  __shared__ uint64_t sh_row_keys[kMaxCluster][32];
   cg::cluster_group cluster = cg::this_cluster();
-  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int C = 1 << log_c, rank = blockIdx.x & (C - 1);
+  if (C > 1) cluster.barrier_arrive();
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  const int64_t row = blockIdx.x / C;
+  const int64_t row = blockIdx.x >> log_c;
   const T* x = static_cast<const T*>(p.logits) + row * p.ld;
   const uint32_t V = (uint32_t)p.V;
-  const uint32_t shift = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const T* base = x - shift;  // read from its first full chunk on
-  const uint32_t chunks = (V + shift + VEC - 1) / VEC;
-  const uint32_t j0 = (uint32_t)((uint64_t)chunks * rank / C);
-  const uint32_t j1 = (uint32_t)((uint64_t)chunks * (rank + 1) / C);
-  const bool cut_last = (V + shift) % VEC != 0;
+  const uint32_t cut = (uint32_t)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const T* base = x - cut;  // read from its first whole chunk on
+  const uint32_t chunks = (V + cut + VEC - 1) / VEC;
+  const uint32_t j0 = (uint32_t)((uint64_t)chunks * rank >> log_c);
+  const uint32_t j1 = (uint32_t)((uint64_t)chunks * (rank + 1) >> log_c);
+  const bool cut_last = (V + cut) % VEC != 0;
+  pdl_trigger();
+  pdl_wait();
 
   auto cut_chunk = [&](uint32_t j, float* f) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const uint32_t n = j * VEC + i;
-      f[i] = n >= shift && n < V + shift ? to_f32(base[n]) : __int_as_float(0xff800000);
+      f[i] = n >= cut && n < V + cut ? to_f32(base[n]) : minus_inf();
     }
   };
 
   // ---- one pass: this thread's chunks j0 + tid, + NT, ...
-  Soft a = {__int_as_float(0xff800000), 0.0f, 0.0f};
+  Soft a = {minus_inf(), 0.0f, 0.0f};
   uint32_t j = j0 + tid, best = j;
-  if (tid == 0 && j == 0 && j < j1 && shift) {
+  if (tid == 0 && j == 0 && j < j1 && cut) {
     float f[VEC];
     cut_chunk(0, f);
-    add_chunk<T>(a, best, 0, f);
+    add_chunk<VEC>(a, best, 0, f);
     j += NT;
   }
-  const uint32_t full = j1 == chunks && cut_last ? j1 - 1 : j1;  // full chunks end here
+  const uint32_t full = j1 == chunks && cut_last ? j1 - 1 : j1;  // whole chunks end here
   const uint4* v = reinterpret_cast<const uint4*>(base);
-  if (full > 0)
-    for (; j + (U - 1) * NT < full; j += U * NT) {
-      uint4 c[U];
+  for (; j + (U - 1) * NT < full; j += U * NT) {
+    uint4 c[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) c[u] = __ldg(v + j + u * NT);
+    for (int u = 0; u < U; ++u) c[u] = __ldg(v + j + u * NT);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float f[VEC];
-        unpack(c[u], (const T*)nullptr, f);
-        add_chunk<T>(a, best, j + u * NT, f);
-      }
+    for (int u = 0; u < U; ++u) {
+      float f[VEC];
+      unpack(c[u], (const T*)nullptr, f);
+      add_chunk<VEC>(a, best, j + u * NT, f);
     }
+  }
   for (; j < full; j += NT) {
     float f[VEC];
     unpack(__ldg(v + j), (const T*)nullptr, f);
-    add_chunk<T>(a, best, j, f);
+    add_chunk<VEC>(a, best, j, f);
   }
   if (j < j1) {
     float f[VEC];
     cut_chunk(j, f);
-    add_chunk<T>(a, best, j, f);
+    add_chunk<VEC>(a, best, j, f);
   }
   const bool any = j0 + tid < j1;
 
-  // ---- the CTA's sums, in warp 0's lane 0
-  Soft w = a;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Soft b = {__shfl_down_sync(kFull, w.m, o), __shfl_down_sync(kFull, w.s, o),
-                    __shfl_down_sync(kFull, w.d, o)};
-    w = join(w, b);
-  }
+  // ---- the warps' sums
+  const Soft w = warp_join(a);
   if (lane == 0) sh_soft[wid] = w;
-  if (tid == 0) sh_count = 0;
+  if (tid == 0) sh_count = sh_found = 0;
 
   // ---- the CTA's first `top` keys, in warp 0
   uint64_t keys = 0;
   if (p.top > 0) {
     const uint64_t mine = any ? key_of(a.m, best) : 0;
-    uint64_t b = cta_merge<NW>(warp_sort(mine), sh_keys);
-    if (wid == 0) {
-      const uint64_t bound = __shfl_sync(kFull, b, p.top - 1);
-      if (lane == 0) sh_bound = bound;
-    }
+    const uint64_t b = cta_merge<NW>(warp_sort(mine), sh_keys);
+    if (wid == 0 && lane == p.top - 1) sh_bound = b;
     __syncthreads();
     const uint64_t bound = sh_bound;  // 0: fewer threads than `top` have logits
     if (any && mine >= bound) sh_flagged[atomicAdd(&sh_count, 1)] = tid;
     __syncthreads();
     const int count = sh_count;
     const uint32_t bound_x = (uint32_t)(bound >> 32), bound_j = ~(uint32_t)bound;
-    for (int f = wid; f < count; f += NW) {
-      const uint32_t t = (uint32_t)sh_flagged[f];
-      // lane's element of the thread's chunks: VEC lanes a chunk
-      for (uint32_t jb = j0 + t; jb < j1; jb += 32 / VEC * NT) {
-        const uint64_t jj = (uint64_t)jb + (uint64_t)(lane / VEC) * NT;
-        const uint32_t n = (uint32_t)jj * VEC + lane % VEC;
-        uint64_t key = 0;
-        if (jj < j1 && n >= shift && n < V + shift) {
-          const float e = to_f32(base[n]);
-          const uint32_t o = ordered(e);
-          if (o > bound_x || (o == bound_x && jj <= bound_j)) key = key_of(e, n - shift);
+    // key of this lane's element of chunk jb + i * NT (VEC lanes a chunk), 0
+    // where it does not pass the bound
+    auto key_at = [&](uint32_t jb) -> uint64_t {
+      const uint64_t jj = (uint64_t)jb + (uint64_t)(lane / VEC) * NT;
+      const uint32_t n = (uint32_t)jj * VEC + lane % VEC;
+      if (jj >= j1 || n < cut || n >= V + cut) return 0;
+      const float e = to_f32(base[n]);
+      const uint32_t o = ordered(e);
+      return o > bound_x || (o == bound_x && jj <= bound_j) ? key_of(e, n - cut) : 0;
+    };
+    for (int f = wid; f < count; f += NW)
+      for (uint32_t jb = j0 + (uint32_t)sh_flagged[f]; jb < j1; jb += 32 / VEC * NT) {
+        const uint64_t key = key_at(jb);
+        if (key) {
+          const int at = atomicAdd(&sh_found, 1);
+          if (at < kMaxCandidates) sh_candidates[at] = key;
         }
-        const uint64_t last = __shfl_sync(kFull, keys, p.top - 1);
-        if (__any_sync(kFull, key > last)) keys = warp_merge(keys, warp_sort(key));
       }
+    __syncthreads();
+    const int found = sh_found;
+    if (found <= 32) {
+      if (wid == 0) keys = warp_sort(lane < found ? sh_candidates[lane] : 0);
+    } else {
+      if (found <= kMaxCandidates) {
+        for (int at = wid * 32; at < found; at += NW * 32) {
+          const uint64_t key = at + lane < found ? sh_candidates[at + lane] : 0;
+          keys = warp_merge(keys, warp_sort(key));
+        }
+      } else {  // the largest logits lie close together: sorted as they are read
+        for (int f = wid; f < count; f += NW)
+          for (uint32_t jb = j0 + (uint32_t)sh_flagged[f]; jb < j1; jb += 32 / VEC * NT) {
+            const uint64_t key = key_at(jb);
+            const uint64_t last = __shfl_sync(kFull, keys, p.top - 1);
+            if (__any_sync(kFull, key > last)) keys = warp_merge(keys, warp_sort(key));
+          }
+      }
+      keys = cta_merge<NW>(keys, sh_keys);
     }
-    __syncthreads();  // cta_merge above is done with sh_keys
-    keys = cta_merge<NW>(keys, sh_keys);
   }
   __syncthreads();
-  if (wid == 0) {
-    w = lane < NW ? sh_soft[lane] : Soft{__int_as_float(0xff800000), 0.0f, 0.0f};
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const Soft b = {__shfl_down_sync(kFull, w.m, o), __shfl_down_sync(kFull, w.s, o),
-                      __shfl_down_sync(kFull, w.d, o)};
-      w = join(w, b);
-    }
-  }
 
   // ---- the row's, in the first CTA's warp 0
-  if (C > 1) {
-    if (wid == 0) {
-      sh_keys[0][lane] = keys;
-      if (lane == 0) sh_soft[0] = w;
+  Soft r = {minus_inf(), 0.0f, 0.0f};
+  if (C > 1) cluster.barrier_wait();  // every CTA of the cluster runs
+  if (wid == 0) {
+    if (lane < NW) r = sh_soft[lane];
+    r = warp_join(r);
+    if (C > 1) {
+      if (lane == 0) *cluster.map_shared_rank(&sh_row[rank], 0) = r;
+      if (p.top > 0) *cluster.map_shared_rank(&sh_row_keys[rank][lane], 0) = keys;
     }
-    cluster.sync();
-    if (rank == 0 && wid == 0)
-      for (int r = 1; r < C; ++r) {
-        w = join(w, *cluster.map_shared_rank(&sh_soft[0], r));
-        if (p.top > 0) keys = warp_merge(keys, cluster.map_shared_rank(&sh_keys[0][0], r)[lane]);
-      }
-    cluster.sync();  // the other CTAs' shared memory has been read
   }
-  if (rank != 0 || wid != 0) return;
-  w.m = __shfl_sync(kFull, w.m, 0);
-  w.s = __shfl_sync(kFull, w.s, 0);
-  w.d = __shfl_sync(kFull, w.d, 0);
+  if (C > 1) {
+    cluster.sync();
+    if (rank != 0) return;
+    if (wid == 0) r = warp_join(lane < C ? sh_row[lane] : Soft{minus_inf(), 0.0f, 0.0f});
+    if (p.top > 0) keys = cta_merge<kMaxCluster>(wid < C ? sh_row_keys[wid][lane] : 0, sh_keys);
+  }
+  if (wid != 0) return;
   // a row whose logits are all -inf has s = 0 and no distribution
-  const float minus_inf = __int_as_float(0xff800000);
-  const float log_s = logf(w.s);
-  auto log_p = [&](float e) { return w.s == 0.0f ? minus_inf : (e - fmaxf(w.m, kLowest)) - log_s; };
+  const float m = fmaxf(r.m, kLowest);
+  const float rest = fabsf(m) <= kWide ? fmaf(m, kLog2E, -shift_of(m)) : 0.0f;
+  const float log2_s = log2f(r.s);
+  auto log_p = [&](float e) {
+    return r.s == 0.0f ? minus_inf() : (e - m) - kLn2 * (log2_s - rest);
+  };
   if (lane == 0) {
     if (p.entropy) {
-      const float h = log_s - w.d / w.s;
-      p.entropy[row] = w.s == 0.0f || h < 0.0f ? 0.0f : h;
+      const float h = kLn2 * (log2_s - r.d / r.s);
+      p.entropy[row] = r.s == 0.0f || h < 0.0f ? 0.0f : h;
     }
     if (p.tokens) {
       const int32_t t = p.tokens[row];
       float lp = 0.0f;
-      if (t >= 0) lp = (uint32_t)t < V ? log_p(to_f32(x[t])) : __int_as_float(0x7fc00000);
+      if (t >= 0) lp = (uint32_t)t < V ? log_p(to_f32(x[t])) : nan_f32();
       p.logprobs[row] = lp;
     }
   }
@@ -288,27 +358,34 @@ __global__ void __launch_bounds__(512)
   }
 }
 
+template <class T, int NT>
+int launch(const TokenLogprobsArgs& p, int log_c, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.T << log_c));
+  cfg.blockDim = dim3(NT);
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 1u << log_c;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, NT>, p, log_c);
+  count_launch();
+  return launch_result(e != cudaSuccess ? e : cudaGetLastError());
+}
+
 template <class T>
 int run(const TokenLogprobsArgs& p, cudaStream_t st) {
   // One CTA a row where the rows fill the GPU; otherwise the row is split, as
   // long as every thread keeps two chunks.
   const int64_t chunks = (p.V + Chunk<T>::kElems - 1) / Chunk<T>::kElems;
-  int C = 1;
-  while (C < 8 && p.T * C < 148 * 4 && chunks >= (int64_t)C * 2 * 512 * 2) C *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.T * C));
-  cfg.blockDim = dim3(512);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = C;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, p);
-  count_launch();
-  return launch_result(e != cudaSuccess ? e : cudaGetLastError());
+  int l = 0;
+  while (l < 3 && (p.T << l) < 148 * 2 && chunks >= (int64_t)512 * 2 << l) ++l;
+  return launch<T, 256>(p, l, st);
 }
 
 }  // namespace
