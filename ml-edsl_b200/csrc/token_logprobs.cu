@@ -181,6 +181,15 @@ __device__ __forceinline__ void add_chunk(Soft& a, uint32_t& best, uint32_t j, c
   }
 }
 
+template <int VEC>
+__device__ __forceinline__ bool has(const float (&x)[VEC], float m) {
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r |= x[i] == m;
+  return r;
+}
+
+constexpr uint32_t kNoChunk = 0xffffffffu;
 constexpr int kMaxCandidates = 256;
 constexpr int kMaxCluster = 8;
 
@@ -215,47 +224,71 @@ __global__ void __launch_bounds__(NT)
   pdl_trigger();
   pdl_wait();
 
-  auto cut_chunk = [&](uint32_t j, float* f) {
+  // ---- one pass. The cut chunks at the row's ends belong to threads 0 and 32
+  // of the first and the last CTA; the whole ones go round: w0 + tid, + NT, ...
+  const uint32_t w0 = j0 == 0 && cut ? 1 : j0, w1 = j1 == chunks && cut_last ? j1 - 1 : j1;
+  uint32_t edge = kNoChunk;
+  if (tid == 0 && w0 != j0) edge = 0;
+  if (tid == 32 && j1 > w0 && w1 != j1) edge = j1 - 1;
+  float at_edge[VEC];
+  if (edge != kNoChunk) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const uint32_t n = j * VEC + i;
-      f[i] = n >= cut && n < V + cut ? to_f32(base[n]) : minus_inf();
+      const uint32_t n = edge * VEC + i;
+      at_edge[i] = n >= cut && n < V + cut ? to_f32(base[n]) : minus_inf();
     }
-  };
-
-  // ---- one pass: this thread's chunks j0 + tid, + NT, ...
-  Soft a = {minus_inf(), 0.0f, 0.0f};
-  uint32_t j = j0 + tid, best = j;
-  if (tid == 0 && j == 0 && j < j1 && cut) {
-    float f[VEC];
-    cut_chunk(0, f);
-    add_chunk<VEC>(a, best, 0, f);
-    j += NT;
   }
-  const uint32_t full = j1 == chunks && cut_last ? j1 - 1 : j1;  // whole chunks end here
+  Soft a = {minus_inf(), 0.0f, 0.0f};
+  uint32_t j = w0 + tid, best = j;
+  const bool any = j < w1 || edge != kNoChunk;
   const uint4* v = reinterpret_cast<const uint4*>(base);
-  for (; j + (U - 1) * NT < full; j += U * NT) {
-    uint4 c[U];
+  // four chunks on their way while four are added
+  uint4 c[U];
+  bool have = j + (U - 1) * NT < w1;
+  if (have) {
 #pragma unroll
     for (int u = 0; u < U; ++u) c[u] = __ldg(v + j + u * NT);
+  }
+  while (have) {
+    uint4 next[U];
+    const uint32_t jn = j + U * NT;
+    have = jn + (U - 1) * NT < w1;
+    if (have) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = __ldg(v + jn + u * NT);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float f[VEC];
       unpack(c[u], (const T*)nullptr, f);
       add_chunk<VEC>(a, best, j + u * NT, f);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) c[u] = next[u];
+    j = jn;
   }
-  for (; j < full; j += NT) {
-    float f[VEC];
-    unpack(__ldg(v + j), (const T*)nullptr, f);
-    add_chunk<VEC>(a, best, j, f);
+  {  // the last ones, fewer than U
+    uint4 r[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (j + u * NT < w1) r[u] = __ldg(v + j + u * NT);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (j + u * NT < w1) {
+        float f[VEC];
+        unpack(r[u], (const T*)nullptr, f);
+        add_chunk<VEC>(a, best, j + u * NT, f);
+      }
   }
-  if (j < j1) {
-    float f[VEC];
-    cut_chunk(j, f);
-    add_chunk<VEC>(a, best, j, f);
+  if (edge != kNoChunk) {
+    const float before = a.m;
+    uint32_t first = best;
+    add_chunk<VEC>(a, first, edge, at_edge);
+    // where two chunks hold the maximum, the lower one
+    if (first == edge || w0 + tid >= w1 || (edge < best && a.m == before && has(at_edge, a.m)))
+      first = edge;
+    best = first;
   }
-  const bool any = j0 + tid < j1;
 
   // ---- the warps' sums
   const Soft w = warp_join(a);
@@ -274,24 +307,30 @@ __global__ void __launch_bounds__(NT)
     __syncthreads();
     const int count = sh_count;
     const uint32_t bound_x = (uint32_t)(bound >> 32), bound_j = ~(uint32_t)bound;
-    // key of this lane's element of chunk jb + i * NT (VEC lanes a chunk), 0
-    // where it does not pass the bound
-    auto key_at = [&](uint32_t jb) -> uint64_t {
-      const uint64_t jj = (uint64_t)jb + (uint64_t)(lane / VEC) * NT;
-      const uint32_t n = (uint32_t)jj * VEC + lane % VEC;
-      if (jj >= j1 || n < cut || n >= V + cut) return 0;
+    // key of the element n of the row's chunks (n - cut of the row), 0 where it
+    // does not pass the bound
+    auto key_at = [&](uint32_t n) -> uint64_t {
+      if (n < cut || n >= V + cut) return 0;
       const float e = to_f32(base[n]);
       const uint32_t o = ordered(e);
-      return o > bound_x || (o == bound_x && jj <= bound_j) ? key_of(e, n - cut) : 0;
+      return o > bound_x || (o == bound_x && n / VEC <= bound_j) ? key_of(e, n - cut) : 0;
+    };
+    // calls fn(key) for all of a flagged thread's elements, a warp's lanes
+    // taking one each
+    auto each = [&](uint32_t t, auto fn) {
+      for (uint32_t jb = w0 + t; jb < w1; jb += 32 / VEC * NT) {
+        const uint64_t jj = (uint64_t)jb + (uint64_t)(lane / VEC) * NT;
+        fn(jj < w1 ? key_at((uint32_t)jj * VEC + lane % VEC) : 0);
+      }
+      if (t == 0 && w0 != j0) fn(lane < VEC ? key_at(lane) : 0);
+      if (t == 32 && j1 > w0 && w1 != j1) fn(lane < VEC ? key_at(w1 * VEC + lane) : 0);
     };
     for (int f = wid; f < count; f += NW)
-      for (uint32_t jb = j0 + (uint32_t)sh_flagged[f]; jb < j1; jb += 32 / VEC * NT) {
-        const uint64_t key = key_at(jb);
-        if (key) {
-          const int at = atomicAdd(&sh_found, 1);
-          if (at < kMaxCandidates) sh_candidates[at] = key;
-        }
-      }
+      each((uint32_t)sh_flagged[f], [&](uint64_t key) {
+        if (!key) return;
+        const int at = atomicAdd(&sh_found, 1);
+        if (at < kMaxCandidates) sh_candidates[at] = key;
+      });
     __syncthreads();
     const int found = sh_found;
     if (found <= 32) {
@@ -304,11 +343,10 @@ __global__ void __launch_bounds__(NT)
         }
       } else {  // the largest logits lie close together: sorted as they are read
         for (int f = wid; f < count; f += NW)
-          for (uint32_t jb = j0 + (uint32_t)sh_flagged[f]; jb < j1; jb += 32 / VEC * NT) {
-            const uint64_t key = key_at(jb);
+          each((uint32_t)sh_flagged[f], [&](uint64_t key) {
             const uint64_t last = __shfl_sync(kFull, keys, p.top - 1);
             if (__any_sync(kFull, key > last)) keys = warp_merge(keys, warp_sort(key));
-          }
+          });
       }
       keys = cta_merge<NW>(keys, sh_keys);
     }
