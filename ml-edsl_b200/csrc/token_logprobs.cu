@@ -17,11 +17,12 @@
 // first one's shared memory: no scratch in device memory, one launch.
 //
 // The `top` most probable tokens need no second pass over the row. The k-th
-// largest of the threads' maxima is a lower bound of the k-th largest logit,
-// and only the k threads at or above it hold logits that can be among the
-// first k: these threads' logits are read again (L2), and the few that pass
-// the bound are sorted. Order: by logit, then the lowest index; NaN ranks as
-// -inf.
+// largest of 32 groups' maxima (a group: the threads of one lane number) is a
+// lower bound of the k-th largest logit, and only threads whose own maximum
+// reaches it hold logits that can be among the first k: their warps read these
+// threads' logits again (L2), and each of the few that reach the bound finds
+// its place by counting the larger ones. Order: by logit, then the lowest
+// index; NaN ranks as -inf.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <algorithm>
@@ -146,9 +147,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// VEC logits, chunk j of the row, into a thread's sums.
+// VEC logits into a thread's sums.
 template <int VEC>
-__device__ __forceinline__ void add_chunk(Soft& a, uint32_t& best, uint32_t j, const float* x) {
+__device__ __forceinline__ void add_chunk(Soft& a, const float* x) {
   float cm = x[0];
 #pragma unroll
   for (int i = 1; i < VEC; ++i) cm = max_nan(cm, x[i]);
@@ -156,10 +157,7 @@ __device__ __forceinline__ void add_chunk(Soft& a, uint32_t& best, uint32_t j, c
     float m = a.m;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) m = fmaxf(m, x[i]);
-    if (m > a.m) {
-      rescale(a, m);
-      best = j;
-    }
+    if (m > a.m) rescale(a, m);
     if (cm != cm || cm == __int_as_float(0x7f800000)) a.s = nan_f32();  // no distribution
   }
   const float m = fmaxf(a.m, kLowest);
@@ -181,33 +179,25 @@ __device__ __forceinline__ void add_chunk(Soft& a, uint32_t& best, uint32_t j, c
   }
 }
 
-template <int VEC>
-__device__ __forceinline__ bool has(const float (&x)[VEC], float m) {
-  bool r = false;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) r |= x[i] == m;
-  return r;
-}
-
 constexpr uint32_t kNoChunk = 0xffffffffu;
 constexpr int kMaxCandidates = 256;
 constexpr int kMaxCluster = 8;
 
-// Chunk j of a row: its elements [j * VEC - shift, + VEC), which start on 16
+// Chunk j of a row: its elements [j * VEC - cut, + VEC), which start on 16
 // bytes; the row's first and last chunk may be cut.
 template <class T, int NT>
 __global__ void __launch_bounds__(NT)
     token_logprobs_kernel(const __grid_constant__ TokenLogprobsArgs p, int log_c) {
   constexpr int VEC = Chunk<T>::kElems, NW = NT / 32, U = 4;
   __shared__ Soft sh_soft[NW];
+  __shared__ uint32_t sh_max[NT];
+  __shared__ uint8_t sh_lanes[NW][32];
   __shared__ uint64_t sh_keys[NW][32];
   __shared__ uint64_t sh_candidates[kMaxCandidates];
-  __shared__ int sh_flagged[kMaxTop];
-  __shared__ int sh_count, sh_found;
-  __shared__ uint64_t sh_bound;
+  __shared__ int sh_found;
   // what the cluster's CTAs send to the first one
   __shared__ Soft sh_row[kMaxCluster];
-  __shared__ uint64_t sh_row_keys[kMaxCluster][32];
+  __shared__ uint64_t sh_row_keys[kMaxCluster * kMaxTop];
   cg::cluster_group cluster = cg::this_cluster();
   const int C = 1 << log_c, rank = blockIdx.x & (C - 1);
   if (C > 1) cluster.barrier_arrive();
@@ -238,8 +228,15 @@ __global__ void __launch_bounds__(NT)
       at_edge[i] = n >= cut && n < V + cut ? to_f32(base[n]) : minus_inf();
     }
   }
+  // the given token's logit, for the end
+  int32_t token = -1;
+  float given = 0.0f;
+  if (rank == 0 && tid == NT - 1 && p.tokens) {
+    token = p.tokens[row];
+    if (token >= 0 && (uint32_t)token < V) given = to_f32(x[token]);
+  }
   Soft a = {minus_inf(), 0.0f, 0.0f};
-  uint32_t j = w0 + tid, best = j;
+  uint32_t j = w0 + tid;
   const bool any = j < w1 || edge != kNoChunk;
   const uint4* v = reinterpret_cast<const uint4*>(base);
   // four chunks on their way while four are added
@@ -261,7 +258,7 @@ __global__ void __launch_bounds__(NT)
     for (int u = 0; u < U; ++u) {
       float f[VEC];
       unpack(c[u], (const T*)nullptr, f);
-      add_chunk<VEC>(a, best, j + u * NT, f);
+      add_chunk<VEC>(a, f);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) c[u] = next[u];
@@ -277,100 +274,137 @@ __global__ void __launch_bounds__(NT)
       if (j + u * NT < w1) {
         float f[VEC];
         unpack(r[u], (const T*)nullptr, f);
-        add_chunk<VEC>(a, best, j + u * NT, f);
+        add_chunk<VEC>(a, f);
       }
   }
-  if (edge != kNoChunk) {
-    const float before = a.m;
-    uint32_t first = best;
-    add_chunk<VEC>(a, first, edge, at_edge);
-    // where two chunks hold the maximum, the lower one
-    if (first == edge || w0 + tid >= w1 || (edge < best && a.m == before && has(at_edge, a.m)))
-      first = edge;
-    best = first;
-  }
+  if (edge != kNoChunk) add_chunk<VEC>(a, at_edge);
 
   // ---- the warps' sums
+  const uint32_t mine = any ? ordered(a.m) : 0;
   const Soft w = warp_join(a);
   if (lane == 0) sh_soft[wid] = w;
-  if (tid == 0) sh_count = sh_found = 0;
-
-  // ---- the CTA's first `top` keys, in warp 0
-  uint64_t keys = 0;
-  if (p.top > 0) {
-    const uint64_t mine = any ? key_of(a.m, best) : 0;
-    const uint64_t b = cta_merge<NW>(warp_sort(mine), sh_keys);
-    if (wid == 0 && lane == p.top - 1) sh_bound = b;
-    __syncthreads();
-    const uint64_t bound = sh_bound;  // 0: fewer threads than `top` have logits
-    if (any && mine >= bound) sh_flagged[atomicAdd(&sh_count, 1)] = tid;
-    __syncthreads();
-    const int count = sh_count;
-    const uint32_t bound_x = (uint32_t)(bound >> 32), bound_j = ~(uint32_t)bound;
-    // key of the element n of the row's chunks (n - cut of the row), 0 where it
-    // does not pass the bound
-    auto key_at = [&](uint32_t n) -> uint64_t {
-      if (n < cut || n >= V + cut) return 0;
-      const float e = to_f32(base[n]);
-      const uint32_t o = ordered(e);
-      return o > bound_x || (o == bound_x && n / VEC <= bound_j) ? key_of(e, n - cut) : 0;
-    };
-    // calls fn(key) for all of a flagged thread's elements, a warp's lanes
-    // taking one each
-    auto each = [&](uint32_t t, auto fn) {
-      for (uint32_t jb = w0 + t; jb < w1; jb += 32 / VEC * NT) {
-        const uint64_t jj = (uint64_t)jb + (uint64_t)(lane / VEC) * NT;
-        fn(jj < w1 ? key_at((uint32_t)jj * VEC + lane % VEC) : 0);
-      }
-      if (t == 0 && w0 != j0) fn(lane < VEC ? key_at(lane) : 0);
-      if (t == 32 && j1 > w0 && w1 != j1) fn(lane < VEC ? key_at(w1 * VEC + lane) : 0);
-    };
-    for (int f = wid; f < count; f += NW)
-      each((uint32_t)sh_flagged[f], [&](uint64_t key) {
-        if (!key) return;
-        const int at = atomicAdd(&sh_found, 1);
-        if (at < kMaxCandidates) sh_candidates[at] = key;
-      });
-    __syncthreads();
-    const int found = sh_found;
-    if (found <= 32) {
-      if (wid == 0) keys = warp_sort(lane < found ? sh_candidates[lane] : 0);
-    } else {
-      if (found <= kMaxCandidates) {
-        for (int at = wid * 32; at < found; at += NW * 32) {
-          const uint64_t key = at + lane < found ? sh_candidates[at + lane] : 0;
-          keys = warp_merge(keys, warp_sort(key));
-        }
-      } else {  // the largest logits lie close together: sorted as they are read
-        for (int f = wid; f < count; f += NW)
-          each((uint32_t)sh_flagged[f], [&](uint64_t key) {
-            const uint64_t last = __shfl_sync(kFull, keys, p.top - 1);
-            if (__any_sync(kFull, key > last)) keys = warp_merge(keys, warp_sort(key));
-          });
-      }
-      keys = cta_merge<NW>(keys, sh_keys);
-    }
-  }
+  sh_max[tid] = mine;
+  if (tid == 0) sh_found = 0;
   __syncthreads();
 
-  // ---- the row's, in the first CTA's warp 0
-  Soft r = {minus_inf(), 0.0f, 0.0f};
-  if (C > 1) cluster.barrier_wait();  // every CTA of the cluster runs
-  if (wid == 0) {
-    if (lane < NW) r = sh_soft[lane];
-    r = warp_join(r);
-    if (C > 1) {
-      if (lane == 0) *cluster.map_shared_rank(&sh_row[rank], 0) = r;
-      if (p.top > 0) *cluster.map_shared_rank(&sh_row_keys[rank][lane], 0) = keys;
+  // ---- the CTA's candidates for the first `top`
+  if (p.top > 0) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) most = max(most, sh_max[i * 32 + lane]);
+    int place = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint32_t o = __shfl_sync(kFull, most, i);
+      place += o > most || (o == most && i < lane);
+    }
+    const unsigned at = __ballot_sync(kFull, place == p.top - 1);
+    // 0: fewer than `top` groups have logits, and all of them pass
+    const uint32_t bound = __shfl_sync(kFull, most, __ffs(at) - 1);
+    const float least = unordered(bound);
+    const bool flagged = any && mine >= bound;
+    const unsigned mask = __ballot_sync(kFull, flagged);
+    if (flagged) sh_lanes[wid][__popc(mask & ((1u << lane) - 1))] = (uint8_t)lane;
+    __syncwarp();
+    const uint32_t per = (w1 - w0 + NT - 1) / NT;  // whole chunks of a thread, at most
+    const uint32_t work = (w1 > w0 ? per : 0) * __popc(mask);
+    const bool first_edge = wid == 0 && (mask & 1) && w0 != j0;
+    const bool last_edge = wid == 1 && (mask & 1) && j1 > w0 && w1 != j1;
+    // this lane's chunk number q of the warp's flagged threads
+    auto load = [&](uint32_t q, float (&f)[VEC]) -> uint32_t {
+      const uint32_t l = sh_lanes[wid][q / per];
+      const uint64_t jj = (uint64_t)w0 + wid * 32 + l + (uint64_t)(q % per) * NT;
+      if (jj >= w1) return kNoChunk;
+      unpack(__ldg(v + jj), (const T*)nullptr, f);
+      return (uint32_t)jj;
+    };
+    auto load_edge = [&](uint32_t n, float& f) {
+      const bool is = lane < VEC && n >= cut && n < V + cut;
+      if (is) f = to_f32(base[n]);
+      return is;
+    };
+    auto offer = [&](float f, uint32_t n) {
+      const int slot = atomicAdd(&sh_found, 1);
+      if (slot < kMaxCandidates) sh_candidates[slot] = key_of(f, n - cut);
+    };
+    for (uint32_t q = lane; q < work; q += 32) {
+      float f[VEC];
+      const uint32_t jj = load(q, f);
+      if (jj == kNoChunk) continue;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (!(f[i] < least)) offer(f[i], jj * VEC + i);
+    }
+    float f1 = 0.0f;
+    if (first_edge && load_edge(lane, f1) && !(f1 < least)) offer(f1, lane);
+    if (last_edge && load_edge(w1 * VEC + lane, f1) && !(f1 < least)) offer(f1, w1 * VEC + lane);
+    __syncthreads();
+    if (sh_found > kMaxCandidates) {  // many alike: sorted as they are read
+      uint64_t keys = 0;
+      auto insert = [&](uint64_t key) {
+        const uint64_t last = __shfl_sync(kFull, keys, p.top - 1);
+        if (__any_sync(kFull, key > last)) keys = warp_merge(keys, warp_sort(key));
+      };
+      for (uint32_t q0 = 0; q0 < work; q0 += 32) {
+        float f[VEC];
+        const uint32_t jj = q0 + lane < work ? load(q0 + lane, f) : kNoChunk;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          insert(jj != kNoChunk ? key_of(f[i], jj * VEC + i - cut) : 0);
+      }
+      if (first_edge) insert(load_edge(lane, f1) ? key_of(f1, lane - cut) : 0);
+      if (last_edge)
+        insert(load_edge(w1 * VEC + lane, f1) ? key_of(f1, w1 * VEC + lane - cut) : 0);
+      keys = cta_merge<NW>(keys, sh_keys);
+      if (wid == 0) sh_candidates[lane] = keys;
+      if (tid == 0) sh_found = 32;
+      __syncthreads();
     }
   }
+
+  // ---- the row's sums, in the first CTA
+  if (C > 1) cluster.barrier_wait();  // every CTA of the cluster runs
+  if (wid == 0) {
+    const Soft r = warp_join(lane < NW ? sh_soft[lane] : Soft{minus_inf(), 0.0f, 0.0f});
+    if (lane == 0) *(C > 1 ? cluster.map_shared_rank(&sh_row[rank], 0) : &sh_row[0]) = r;
+  }
+  // a candidate's place, by the number of larger ones
+  uint64_t key = 0;
+  int place = 0;
+  const int found = p.top > 0 ? sh_found : 0;
+  if (tid < found) {
+    key = sh_candidates[tid];
+#pragma unroll 8
+    for (int i = 0; i < found; ++i) place += sh_candidates[i] > key;
+  }
   if (C > 1) {
+    if (p.top > 0) {
+      uint64_t* to = cluster.map_shared_rank(&sh_row_keys[rank * p.top], 0);
+      if (key && place < p.top) to[place] = key;
+      if (tid < p.top && tid >= found) to[tid] = 0;
+    }
     cluster.sync();
     if (rank != 0) return;
-    if (wid == 0) r = warp_join(lane < C ? sh_row[lane] : Soft{minus_inf(), 0.0f, 0.0f});
-    if (p.top > 0) keys = cta_merge<kMaxCluster>(wid < C ? sh_row_keys[wid][lane] : 0, sh_keys);
+    // the CTAs' lists are in order: the place by a search in each
+    key = tid < p.top << log_c ? sh_row_keys[tid] : 0;
+    place = 0;
+    if (key) {
+#pragma unroll
+      for (int c = 0; c < kMaxCluster; ++c) {
+        if (c >= C) break;
+        const uint64_t* list = sh_row_keys + c * p.top;
+        int n = 0;  // of the list's that are larger
+#pragma unroll
+        for (int step = kMaxTop; step > 0; step /= 2)
+          if (n + step <= p.top && list[n + step - 1] > key) n += step;
+        place += n;
+      }
+    }
+  } else {
+    __syncthreads();
   }
-  if (wid != 0) return;
+  Soft r = sh_row[0];
+  if (C > 1) r = warp_join(lane < C ? sh_row[lane] : Soft{minus_inf(), 0.0f, 0.0f});
   // a row whose logits are all -inf has s = 0 and no distribution
   const float m = fmaxf(r.m, kLowest);
   const float rest = fabsf(m) <= kWide ? fmaf(m, kLog2E, -shift_of(m)) : 0.0f;
@@ -378,21 +412,20 @@ __global__ void __launch_bounds__(NT)
   auto log_p = [&](float e) {
     return r.s == 0.0f ? minus_inf() : (e - m) - kLn2 * (log2_s - rest);
   };
-  if (lane == 0) {
+  if (tid == NT - 1) {
     if (p.entropy) {
       const float h = kLn2 * (log2_s - r.d / r.s);
       p.entropy[row] = r.s == 0.0f || h < 0.0f ? 0.0f : h;
     }
     if (p.tokens) {
-      const int32_t t = p.tokens[row];
       float lp = 0.0f;
-      if (t >= 0) lp = (uint32_t)t < V ? log_p(to_f32(x[t])) : nan_f32();
+      if (token >= 0) lp = (uint32_t)token < V ? log_p(given) : nan_f32();
       p.logprobs[row] = lp;
     }
   }
-  if (lane < p.top) {
-    p.top_logprobs[row * p.top + lane] = log_p(unordered((uint32_t)(keys >> 32)));
-    p.top_tokens[row * p.top + lane] = (int32_t)~(uint32_t)keys;
+  if (key && place < p.top) {
+    p.top_logprobs[row * p.top + place] = log_p(unordered((uint32_t)(key >> 32)));
+    p.top_tokens[row * p.top + place] = (int32_t)~(uint32_t)key;
   }
 }
 
