@@ -15,6 +15,7 @@
 #include <cstdint>
 #include "dtype.cuh"
 #include "kernels.h"
+#include "ptx.cuh"
 
 namespace b200 {
 
@@ -147,93 +148,140 @@ __device__ __forceinline__ Factor factor(float ss, float N, float eps, Fn square
   return {c, 1.0f / sqrtf(squares(c) / N + eps * c * c)};
 }
 
-// One row by TPR threads, E chunks of 16 bytes a thread: chunk e * TPR + t of
-// the row is thread t's e-th. The row is read once and stays in registers.
+// A chunk of x (and of r) as it lies in memory, or as floats where it has to be
+// read element by element.
+template <class T, bool AL>
+struct RawChunk {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* row, int64_t n, int64_t N) {
+    constexpr int VEC = Chunk<T>::kElems;
+    if (n + VEC <= N) {
+      v = *reinterpret_cast<const uint4*>(row + n);
+    } else {
+      float f[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) f[i] = n + i < N ? to_f32(row[n + i]) : 0.0f;
+      v = pack(f, (const T*)nullptr);  // the values are T's: nothing is rounded
+    }
+  }
+  __device__ __forceinline__ void floats(float* f) const { unpack(v, (const T*)nullptr, f); }
+};
+template <class T>
+struct RawChunk<T, false> {
+  float v[Chunk<T>::kElems];
+  __device__ __forceinline__ void load(const T* row, int64_t n, int64_t N) {
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::kElems; ++i) v[i] = n + i < N ? to_f32(row[n + i]) : 0.0f;
+  }
+  __device__ __forceinline__ void floats(float* f) const {
+#pragma unroll
+    for (int i = 0; i < Chunk<T>::kElems; ++i) f[i] = v[i];
+  }
+};
+
+// Rows by TPR threads each, E chunks of 16 bytes a thread: chunk e * TPR + t of
+// a row is thread t's e-th. A row is read once and stays in registers; the next
+// row of the CTA is on its way while one is summed, scaled and stored.
 template <class T, int TPR, int E, bool AL>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
     rms_norm_kernel(const __grid_constant__ RmsNormArgs p) {
   constexpr int VEC = Chunk<T>::kElems;
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-  __shared__ float sh[3][32];
+  __shared__ float sh[2][3][32];  // in turn, for one row and the next
   const int t = threadIdx.x % TPR;
-  const int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
-  if (m >= p.M) return;  // whole warps: TPR is 32 where a CTA has several rows
-  const T* x = static_cast<const T*>(p.X) + m * p.ldx;
-  const T* r = p.R ? static_cast<const T*>(p.R) + m * p.ldr : nullptr;
-
-  float h[E][VEC];
-  float ss = 0.0f;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  pdl_trigger();
+  pdl_wait();
+  RawChunk<T, AL> xs[E], rs[E];
+  auto load_row = [&](int64_t m) {
+    const T* x = static_cast<const T*>(p.X) + m * p.ldx;
 #pragma unroll
-  for (int e = 0; e < E; ++e) load_chunk<T, AL>(x, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
-  if (r) {
+    for (int e = 0; e < E; ++e) xs[e].load(x, (int64_t)(e * TPR + t) * VEC, p.N);
+    if (p.R) {
+      const T* r = static_cast<const T*>(p.R) + m * p.ldr;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float f[VEC];
-      load_chunk<T, AL>(r, (int64_t)(e * TPR + t) * VEC, p.N, f);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[e][i] += f[i];
+      for (int e = 0; e < E; ++e) rs[e].load(r, (int64_t)(e * TPR + t) * VEC, p.N);
     }
-  }
+  };
+  if (m < p.M) load_row(m);
+  // rows of whole warps: TPR is 32 where a CTA has several
+  for (int odd = 0; m < p.M; m += step, odd ^= 1) {
+    float h[E][VEC];
 #pragma unroll
-  for (int e = 0; e < E; ++e)
+    for (int e = 0; e < E; ++e) xs[e].floats(h[e]);
+    if (p.R) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) ss = fmaf(h[e][i], h[e][i], ss);
-  ss = row_reduce<Sum, TPR>(ss, sh[0]);
-  const Factor f = factor(ss, (float)p.N, p.eps, [&](float c) {
-    float s = 0.0f;
+      for (int e = 0; e < E; ++e) {
+        float f[VEC];
+        rs[e].floats(f);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) h[e][i] += f[i];
+      }
+    }
+    if (m + step < p.M) load_row(m + step);
+    float ss = 0.0f;
+#pragma unroll
     for (int e = 0; e < E; ++e)
-      for (int i = 0; i < VEC; ++i) s = fmaf(h[e][i] * c, h[e][i] * c, s);
-    return row_reduce<Sum, TPR>(s, sh[1]);
-  });
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) ss = fmaf(h[e][i], h[e][i], ss);
+    ss = row_reduce<Sum, TPR>(ss, sh[odd][0]);
+    const Factor f = factor(ss, (float)p.N, p.eps, [&](float c) {
+      float s = 0.0f;
+      for (int e = 0; e < E; ++e)
+        for (int i = 0; i < VEC; ++i) s = fmaf(h[e][i] * c, h[e][i] * c, s);
+      return row_reduce<Sum, TPR>(s, sh[odd][1]);
+    });
 
-  if (p.H) {
-    T* hrow = static_cast<T*>(p.H) + m * p.ldh;
+    if (p.H) {
+      T* hrow = static_cast<T*>(p.H) + m * p.ldh;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      store_chunk<T, AL>(hrow, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float w[VEC];
-    load_weight<T, AL>(p, (int64_t)(e * TPR + t) * VEC, w);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) h[e][i] = h[e][i] * f.pre * f.inv * w[i];
-  }
-  if (!p.scales) {
-    T* y = static_cast<T*>(p.Y) + m * p.ldy;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      store_chunk<T, AL>(y, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
-    return;
-  }
-  uint8_t* q = static_cast<uint8_t*>(p.Y) + m * p.ldy;
-  float* s = p.scales + m * p.lds;
-  float most[E];
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    most[e] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) most[e] = fmaxf(most[e], fabsf(h[e][i]));
-  }
-  if (p.group == 0) {
-    float all = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) all = fmaxf(all, most[e]);
-    all = row_reduce<Max, TPR>(all, sh[2]);
-    const float scale = scale_of(all);
-    if (t == 0) s[0] = scale;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      store_codes<VEC, AL>(q, (int64_t)(e * TPR + t) * VEC, p.N, h[e], all, scale);
-  } else {
-    const int lanes = p.group / VEC;
+      for (int e = 0; e < E; ++e)
+        store_chunk<T, AL>(hrow, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
+    }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int64_t n = (int64_t)(e * TPR + t) * VEC;
-      const float gm = group_max(most[e], lanes);
-      const float scale = scale_of(gm);
-      if (t % lanes == 0 && n < p.N) s[n / p.group] = scale;
-      store_codes<VEC, AL>(q, n, p.N, h[e], gm, scale);
+      float w[VEC];
+      load_weight<T, AL>(p, (int64_t)(e * TPR + t) * VEC, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) h[e][i] = h[e][i] * f.pre * f.inv * w[i];
+    }
+    if (!p.scales) {
+      T* y = static_cast<T*>(p.Y) + m * p.ldy;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        store_chunk<T, AL>(y, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
+      continue;
+    }
+    uint8_t* q = static_cast<uint8_t*>(p.Y) + m * p.ldy;
+    float* s = p.scales + m * p.lds;
+    float most[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      most[e] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) most[e] = fmaxf(most[e], fabsf(h[e][i]));
+    }
+    if (p.group == 0) {
+      float all = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) all = fmaxf(all, most[e]);
+      all = row_reduce<Max, TPR>(all, sh[odd][2]);
+      const float scale = scale_of(all);
+      if (t == 0) s[0] = scale;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        store_codes<VEC, AL>(q, (int64_t)(e * TPR + t) * VEC, p.N, h[e], all, scale);
+    } else {
+      const int lanes = p.group / VEC;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int64_t n = (int64_t)(e * TPR + t) * VEC;
+        const float gm = group_max(most[e], lanes);
+        const float scale = scale_of(gm);
+        if (t % lanes == 0 && n < p.N) s[n / p.group] = scale;
+        store_codes<VEC, AL>(q, n, p.N, h[e], gm, scale);
+      }
     }
   }
 }
@@ -247,6 +295,8 @@ __global__ void __launch_bounds__(1024)
   __shared__ float sh[3][32];
   const int t = threadIdx.x;
   const int64_t m = blockIdx.x;
+  pdl_trigger();
+  pdl_wait();
   const T* x = static_cast<const T*>(p.X) + m * p.ldx;
   const T* r = p.R ? static_cast<const T*>(p.R) + m * p.ldr : nullptr;
   const int64_t chunks = (p.N + VEC - 1) / VEC;
@@ -313,28 +363,53 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// Launches `kernel`, which may start early (it waits for the kernel before it
+// where it first reads memory).
+template <class Kernel>
+cudaError_t launch_kernel(Kernel kernel, unsigned grid, int threads, const RmsNormArgs& p,
+                          cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <class T, int TPR, int E, bool AL>
-void launch(const RmsNormArgs& p, cudaStream_t st) {
-  constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
-  rms_norm_kernel<T, TPR, E, AL>
-      <<<(unsigned)((p.M + ROWS - 1) / ROWS), TPR < 128 ? 128 : TPR, 0, st>>>(p);
+cudaError_t launch(const RmsNormArgs& p, cudaStream_t st) {
+  constexpr int ROWS = TPR < 128 ? 128 / TPR : 1, THREADS = TPR < 128 ? 128 : TPR;
+  auto kernel = rms_norm_kernel<T, TPR, E, AL>;
+  // as many CTAs as fit, each with the rows that fall to it
+  static const int per_sm = [&] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, THREADS, 0) == cudaSuccess && n
+               ? n
+               : 1;
+  }();
+  const int64_t grid = std::min<int64_t>((p.M + ROWS - 1) / ROWS, (int64_t)148 * per_sm);
+  return launch_kernel(kernel, (unsigned)grid, THREADS, p, st);
 }
 
 template <class T, bool AL>
-void dispatch(const RmsNormArgs& p, cudaStream_t st) {
+cudaError_t dispatch(const RmsNormArgs& p, cudaStream_t st) {
   const int64_t c = (p.N + Chunk<T>::kElems - 1) / Chunk<T>::kElems;
-  if (c <= 32) launch<T, 32, 1, AL>(p, st);
-  else if (c <= 128) launch<T, 32, 4, AL>(p, st);
-  else if (c <= 256) launch<T, 128, 2, AL>(p, st);
-  else if (c <= 512) launch<T, 256, 2, AL>(p, st);
-  else if (c <= 1024) launch<T, 512, 2, AL>(p, st);
-  else if (c <= 2048) launch<T, 512, 4, AL>(p, st);
-  else if (c <= 4096) launch<T, 1024, 4, AL>(p, st);
-  else rms_norm_long_kernel<T, AL><<<(unsigned)p.M, 1024, 0, st>>>(p);
+  if (c <= 32) return launch<T, 32, 1, AL>(p, st);
+  if (c <= 128) return launch<T, 32, 4, AL>(p, st);
+  if (c <= 256) return launch<T, 128, 2, AL>(p, st);
+  if (c <= 512) return launch<T, 256, 2, AL>(p, st);
+  if (c <= 1024) return launch<T, 512, 2, AL>(p, st);
+  if (c <= 2048) return launch<T, 512, 4, AL>(p, st);
+  if (c <= 4096) return launch<T, 1024, 4, AL>(p, st);
+  return launch_kernel(rms_norm_long_kernel<T, AL>, (unsigned)p.M, 1024, p, st);
 }
 
 template <class T>
-void dispatch_aligned(const RmsNormArgs& p, cudaStream_t st) {
+cudaError_t dispatch_aligned(const RmsNormArgs& p, cudaStream_t st) {
   auto ok = [](const void* q, int64_t ld, int64_t elems, int bytes) {
     return (reinterpret_cast<uintptr_t>(q) % bytes) == 0 && ld % elems == 0;
   };
@@ -342,17 +417,17 @@ void dispatch_aligned(const RmsNormArgs& p, cudaStream_t st) {
   const bool al = ok(p.X, p.ldx, VEC, 16) && (!p.R || ok(p.R, p.ldr, VEC, 16)) &&
                   (!p.H || ok(p.H, p.ldh, VEC, 16)) && (!p.w || ok(p.w, VEC, VEC, 16)) &&
                   (p.scales ? ok(p.Y, p.ldy, VEC, VEC) : ok(p.Y, p.ldy, VEC, 16));
-  al ? dispatch<T, true>(p, st) : dispatch<T, false>(p, st);
+  return al ? dispatch<T, true>(p, st) : dispatch<T, false>(p, st);
 }
 
 }  // namespace
 
 int rms_norm(const RmsNormArgs& p, int dtype, cudaStream_t st) {
-  if (dtype == kF32) dispatch_aligned<float>(p, st);
-  else if (dtype == kBF16) dispatch_aligned<bf16>(p, st);
-  else dispatch_aligned<f16>(p, st);
+  const cudaError_t e = dtype == kF32    ? dispatch_aligned<float>(p, st)
+                        : dtype == kBF16 ? dispatch_aligned<bf16>(p, st)
+                                         : dispatch_aligned<f16>(p, st);
   count_launch();
-  return launch_result();
+  return launch_result(e != cudaSuccess ? e : cudaGetLastError());
 }
 
 }  // namespace b200
