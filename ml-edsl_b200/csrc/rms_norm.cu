@@ -70,7 +70,9 @@ template <class T, bool AL>
 __device__ __forceinline__ void store_chunk(T* row, int64_t n, int64_t N, const float* f) {
   constexpr int VEC = Chunk<T>::kElems;
   if (AL && n + VEC <= N) {
-    *reinterpret_cast<uint4*>(row + n) = pack(f, (const T*)nullptr);
+    // streaming: outputs do not push the rows that are still to be read out of
+    // L2 (65536x4096 bf16 with residual: 370 -> 357 us; loads gain nothing)
+    __stcs(reinterpret_cast<uint4*>(row + n), pack(f, (const T*)nullptr));
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
