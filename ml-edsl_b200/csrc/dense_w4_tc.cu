@@ -314,24 +314,32 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
   } else {
     // ---- sums: this lane's column of W, OWN operand columns of it
     const int n = (quarter & 1) * 32 + lane;  // within the strip
-    const int64_t scale_col = strip * p.groups * 64 + column_place(n);
-    auto scale_of_unit = [&](int u) {
-      const int k = b0 * kBlockK + u * UNIT;
-      return live && u < units
-                 ? load_as_f32(p.scales, a.w.s_dtype, scale_col + (int64_t)p.group_of(k) * 64)
-                 : 0.0f;
+    // their scales, asked for a stage ahead; bits, so that nothing waits for
+    // them before they are used (past the last unit or strip: the last again)
+    const bool s32 = a.w.s_dtype == kF32;
+    const int64_t last_strip = (a.w.N - 1) / kStripN;
+    const int64_t scale_col = min(strip, last_strip) * p.groups * 64 + column_place(n);
+    auto scale_bits = [&](int u) -> uint32_t {
+      const int k = b0 * kBlockK + max(0, min(u, units - 1)) * UNIT;
+      const int64_t at = scale_col + (int64_t)p.group_of(min(k, K - 1)) * 64;
+      return s32 ? __ldg(reinterpret_cast<const uint32_t*>(p.scales) + at)
+                 : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p.scales) + at);
     };
-    float next[S::kUnits];
+    uint32_t next[S::kUnits];
+    if (units > 0) {
 #pragma unroll
-    for (int j = 0; j < S::kUnits; ++j) next[j] = scale_of_unit(j);
+      for (int j = 0; j < S::kUnits; ++j) next[j] = scale_bits(j);
+    }
     for (int t = 0; t < stages; ++t) {
       const int s = t % STAGES;
       float scale[S::kUnits];
 #pragma unroll
-      for (int j = 0; j < S::kUnits; ++j) {
-        scale[j] = next[j];
-        next[j] = scale_of_unit((t + 1) * S::kUnits + j);
-      }
+      for (int j = 0; j < S::kUnits; ++j)
+        scale[j] = s32                        ? __uint_as_float(next[j])
+                   : a.w.s_dtype == kBF16     ? __uint_as_float(next[j] << 16)
+                                              : __half2float(__ushort_as_half((unsigned short)next[j]));
+#pragma unroll
+      for (int j = 0; j < S::kUnits; ++j) next[j] = scale_bits((t + 1) * S::kUnits + j);
       if (!mbar_wait_long(&bar->done[s], (t / STAGES) & 1, status, kDevTimeoutAccum, abort_flag))
         break;
       tc_fence_after();
