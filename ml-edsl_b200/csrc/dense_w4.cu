@@ -29,7 +29,6 @@
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <cstdint>
-#include <cstdlib>
 #include "w4.cuh"
 
 namespace cg = cooperative_groups;
@@ -159,24 +158,22 @@ __global__ void w4_dequantize_kernel(const uint32_t* __restrict__ codes, const c
 
 // ------------------------------------------------------------------ product
 
-// Few rows: a CTA has one strip of 64 columns and at most 8 * NT operand
-// columns, and its four warps split the blocks of its part of K. Every lane
+// Few rows: a CTA has one strip of 64 columns and at most 8 operand columns,
+// and its four warps split the blocks of its part of K. Every lane
 // copies the codes that it will use itself, kDepth blocks ahead, into shared
 // memory (cp.async), so the loop over K has no barrier; scales and zeros are
 // one block ahead in registers. The activations of the CTA's part of K are
 // staged once, or stage_blocks of K at a time where that takes more than
 // kXBytes. CTAs are small so that several share an SM and the last wave is
 // short; the CTAs of a cluster share K.
-#ifndef W4MINB
-#define W4MINB 4
-#define W4OCC 4
-#endif
 constexpr int kFewWarps = 4;
+constexpr int kFewColumns = 8;  // operand columns of a CTA
 constexpr int kDepth = 4;
 constexpr int kXBytes = 24 * 1024;
+constexpr int kFewCtas = 4;  // an SM: with five, 96 registers spill (1x4096x4096 5.8 -> 6.5 us)
 
-template <int XT, int NT, bool FINE>
-__global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
+template <int XT, bool FINE>
+__global__ void __launch_bounds__(kFewWarps * 32, kFewCtas)
     dense_w4_few_kernel(const __grid_constant__ W4Params p) {
   using X = XRow<XT>;
   using Mma = typename X::Mma;
@@ -276,15 +273,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
 
   char* xsm = ring + kFewWarps * kDepth * 2048;
   const int pitch = p.stage_blocks * 128 + 64;  // bytes of a staged column: 64 mod 128
-  if (cols < NT * 8 && tid < 8)
+  if (cols < kFewColumns && tid < 8)
     *reinterpret_cast<uint4*>(xsm + cols * pitch + tid * 16) = make_uint4(0, 0, 0, 0);
-  float total[MT][NT][4];
+  float total[MT][4];
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) total[i][j][c] = 0.0f;
+    for (int c = 0; c < 4; ++c) total[i][c] = 0.0f;
 
   int b = b0 + wid, slot = 0;
   for (int s0 = b0; s0 < b1; s0 += p.stage_blocks) {
@@ -330,15 +325,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
         if (um[u] < mrows) store_x(um[u], uc[u], e[u]);
     }
     __syncthreads();
-    // operand column j * 8 + g; columns that no row has read zeros
-    const char* xs[NT];
-    int xstep[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const bool is = j * 8 + g < cols;
-      xs[j] = is ? xsm + (j * 8 + g) * pitch + (b - s0) * 128 + t * 16 : xsm + cols * pitch;
-      xstep[j] = is ? kFewWarps * 128 : 0;
-    }
+    // operand column g; columns that no row has read zeros
+    const char* xs = g < cols ? xsm + g * pitch + (b - s0) * 128 + t * 16 : xsm + cols * pitch;
+    const int xstep = g < cols ? kFewWarps * 128 : 0;
     for (; b < s1; b += kFewWarps) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
       uint4 cur[MT];
@@ -357,12 +346,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
       for (int sub = 0; sub < SUBS; ++sub) {
         const int k = b * kBlockK + sub * 32;
         if (FINE && k >= K) break;  // the second half of the last block
-        float acc[MT][NT][4];
+        float acc[MT][4];
 #pragma unroll
         for (int h = FINE ? sub : 0; h < (FINE ? sub + 1 : 2); ++h) {
-          uint4 xb[NT];
-#pragma unroll
-          for (int j = 0; j < NT; ++j) xb[j] = *reinterpret_cast<const uint4*>(xs[j] + h * 64);
+          const uint4 xb = *reinterpret_cast<const uint4*>(xs + h * 64);
 #pragma unroll
           for (int i = 0; i < MT; ++i) {
             const uint2 w = h == 0 ? make_uint2(cur[i].x, cur[i].y) : make_uint2(cur[i].z, cur[i].w);
@@ -373,13 +360,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
               for (int r = 0; r < 4; ++r)
                 f[r] = Mma::sub(and_or((step == 0 ? w.x : w.y) >> (4 * r), 0x000f000fu, Mma::kMagic),
                                 zero[sub][2 * i + (r & 1)]);
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                const uint32_t b0 = step == 0 ? xb[j].x : xb[j].z;
-                const uint32_t b1 = step == 0 ? xb[j].y : xb[j].w;
-                if (step == 0 && (FINE || h == 0)) Mma::mma_first(acc[i][j], f, b0, b1);
-                else Mma::mma(acc[i][j], f, b0, b1);
-              }
+              const uint32_t x0 = step == 0 ? xb.x : xb.z, x1 = step == 0 ? xb.y : xb.w;
+              if (step == 0 && (FINE || h == 0)) Mma::mma_first(acc[i], f, x0, x1);
+              else Mma::mma(acc[i], f, x0, x1);
             }
           }
         }
@@ -387,17 +370,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
         if (XT == kE4M3 && a.x_group > 0) {
           const unsigned xg = (unsigned)k / (unsigned)a.x_group;
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+          for (int c = 0; c < 2; ++c) {
+            const int m = t * 2 + c;
+            const float s = m < mrows ? __ldg(a.x_scales + (m0 + m) * a.ldxs + xg) : 0.0f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const int m = j * 8 + t * 2 + c;
-              const float s = m < mrows ? __ldg(a.x_scales + (m0 + m) * a.ldxs + xg) : 0.0f;
-#pragma unroll
-              for (int i = 0; i < MT; ++i) {
-                acc[i][j][c] *= s;
-                acc[i][j][2 + c] *= s;
-              }
+            for (int i = 0; i < MT; ++i) {
+              acc[i][c] *= s;
+              acc[i][2 + c] *= s;
             }
+          }
         }
         float sc[2 * MT];
         if (s32) {
@@ -411,16 +392,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-              total[i][j][c] = fmaf(acc[i][j][c], sc[2 * i + (c >> 1)], total[i][j][c]);
+          for (int c = 0; c < 4; ++c)
+            total[i][c] = fmaf(acc[i][c], sc[2 * i + (c >> 1)], total[i][c]);
       }
       fetch_scales(b + kFewWarps);
       fetch(slot);
       slot = (slot + 1) & (kDepth - 1);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) xs[j] += xstep[j];
+      xs += xstep;
     }
   }
 
@@ -431,19 +409,17 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
   float* red = reinterpret_cast<float*>(ring);   // [warp][column][64]
   float* recv = reinterpret_cast<float*>(smem);  // [CTA][part][slot]
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
+  for (int c = 0; c < 2; ++c) {
+    const int col = t * 2 + c;
+    if (col < cols) {
+      float* to = red + (wid * kFewColumns + col) * 64 + g;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int col = j * 8 + t * 2 + c;
-      if (col < cols) {
-        float* to = red + (wid * NT * 8 + col) * 64 + g;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          to[i * 16] = total[i][j][c];
-          to[i * 16 + 8] = total[i][j][2 + c];
-        }
+      for (int i = 0; i < MT; ++i) {
+        to[i * 16] = total[i][c];
+        to[i * 16 + 8] = total[i][2 + c];
       }
     }
+  }
   __syncthreads();
   const int outs = mrows * 64;
   const int slots = ((mrows * 2 + C - 1) >> log_c) * 32;  // outputs of a CTA
@@ -452,7 +428,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
     const int col = u >> 6, m = col / X::kParts, q = col - m * X::kParts;
     float v = red[u];
 #pragma unroll
-    for (int k = 1; k < kFewWarps; ++k) v += red[k * NT * 8 * 64 + u];
+    for (int k = 1; k < kFewWarps; ++k) v += red[k * kFewColumns * 64 + u];
     const int chunk = m * 2 + (u >> 5 & 1);
     float* dst = recv + (rank * X::kParts + q) * slots + (chunk >> log_c) * 32 + (u & 31);
     *(C > 1 ? cluster.map_shared_rank(dst, chunk & (C - 1)) : dst) = v;
@@ -488,20 +464,20 @@ __global__ void __launch_bounds__(kFewWarps * 32, W4MINB)
   }
 }
 
-template <int XT, int NT, bool FINE>
+template <int XT, bool FINE>
 int launch_few(W4Params p, cudaStream_t st) {
-  auto kernel = dense_w4_few_kernel<XT, NT, FINE>;
-  p.rows = NT * 8 / XRow<XT>::kParts;
+  auto kernel = dense_w4_few_kernel<XT, FINE>;
+  p.rows = kFewColumns / XRow<XT>::kParts;
   const int64_t tiles = p.a.w.strips();
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
   if (chunks > 65535) return kErrTooLarge;
-  // CTAs that share K: the fewest waves of the GPU's 148 * W4OCC CTAs, each as
+  // CTAs that share K: the fewest waves of the GPU's 148 * kFewCtas CTAs, each as
   // long as a warp's blocks and kFixed of setting up and adding.
   constexpr int kFixed = 4;
   int best = 0;
   int64_t least = INT64_MAX;
   for (int l = 0; l <= 3; ++l) {
-    const int64_t waves = ((tiles * chunks << l) + 148 * W4OCC - 1) / (148 * W4OCC);
+    const int64_t waves = ((tiles * chunks << l) + 148 * kFewCtas - 1) / (148 * kFewCtas);
     const int64_t blocks = (p.kblocks + (kFewWarps << l) - 1) / (kFewWarps << l);
     const int64_t cost = waves * (blocks + kFixed);
     if (cost < least) {
@@ -509,8 +485,6 @@ int launch_few(W4Params p, cudaStream_t st) {
       best = l;
     }
   }
-  static const int force = getenv("W4C") ? atoi(getenv("W4C")) : -1;
-  if (force >= 0) best = force;
   const int C = 1 << best;
   p.log_cluster = best;
   const int64_t mine = (p.kblocks + C - 1) / C;
@@ -543,14 +517,13 @@ int launch_few(W4Params p, cudaStream_t st) {
   return launch_result(e != cudaSuccess ? e : cudaGetLastError());
 }
 
+// Up to 8 operand columns on mma.sync, whose n it is; more on the tensor core
+// (bf16 12x4096x4096: 7.7 us there, 9.7 with two tiles of 8 columns here).
 template <int XT>
 int dispatch(const W4Params& p, int* status, cudaStream_t st) {
-  const bool fine = p.a.w.group == 32 || p.a.x_group == 32;
-  const int64_t cols = p.a.M * XRow<XT>::kParts;
-  static const int most = getenv("W4MOST") ? atoi(getenv("W4MOST")) : 16;
-  if (cols > most) return dense_w4_tc(p, status, st);
-  if (cols <= 8) return fine ? launch_few<XT, 1, true>(p, st) : launch_few<XT, 1, false>(p, st);
-  return fine ? launch_few<XT, 2, true>(p, st) : launch_few<XT, 2, false>(p, st);
+  if (p.a.M * XRow<XT>::kParts > kFewColumns) return dense_w4_tc(p, status, st);
+  return p.a.w.group == 32 || p.a.x_group == 32 ? launch_few<XT, true>(p, st)
+                                                : launch_few<XT, false>(p, st);
 }
 
 unsigned grid_for(int64_t work) {

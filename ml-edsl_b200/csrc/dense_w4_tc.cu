@@ -24,7 +24,6 @@
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <cstdint>
-#include <cstdlib>
 #include "w4.cuh"
 
 namespace cg = cooperative_groups;
@@ -251,40 +250,53 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
         post(t);
       }
     } else {
-      // others pass through registers, asked for one block ahead
-      Raw next[PER];
-      auto load = [&](int i) {
-        if (i >= nb) return;
-        const int64_t k = (int64_t)(b0 + i) * kBlockK + c * 8;
-        if (p.x_aligned && (b0 + i + 1) * kBlockK <= K) {
+      // others pass through registers: blocks whose 64 columns are all there and
+      // aligned are asked for ahead, as many as fit 32 registers, without a
+      // branch that would wait for them
+      constexpr int WORDS = PER * (int)sizeof(Raw) / 4;
+      constexpr int AHEAD = SB >= 4 && 4 * WORDS <= 32 ? 4 : SB >= 2 && 2 * WORDS <= 32 ? 2 : 1;
+      const int whole = p.x_aligned ? min(nb, (K - b0 * kBlockK) / kBlockK) : 0;
+      const char* rows[PER];
 #pragma unroll
-          for (int u = 0; u < PER; ++u)  // rows past the last: the last again
-            next[u] = X::load_whole(x + min(row0 + u * rows_step, mrows - 1) * a.ldx * X::kBytes, k);
-        } else {
+      for (int u = 0; u < PER; ++u)  // rows past the last: the last again
+        rows[u] = x + ((int64_t)min(row0 + u * rows_step, mrows - 1) * a.ldx + b0 * kBlockK + c * 8) *
+                          X::kBytes;
+      Raw ahead[AHEAD][PER];
+      auto load = [&](int i, Raw (&next)[PER]) {
 #pragma unroll
-          for (int u = 0; u < PER; ++u)
-            next[u] = X::load(x + min(row0 + u * rows_step, mrows - 1) * a.ldx * X::kBytes, k, K,
-                              false);
+        for (int u = 0; u < PER; ++u) next[u] = X::load_whole(rows[u], min(i, whole - 1) * kBlockK);
+      };
+      auto put = [&](int i, const Raw (&raw)[PER]) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+          const int m = row0 + u * rows_step;
+          if (m >= mrows) continue;
+          uint4 out[PARTS];
+          X::stage(raw[u], out);
+#pragma unroll
+          for (int q = 0; q < PARTS; ++q)
+            *reinterpret_cast<uint4*>(place(i, m * PARTS + q)) = out[q];
         }
       };
-      load(0);
+      if (whole > 0) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) load(i, ahead[i]);
+      }
       for (int t = 0; t < stages; ++t) {
         if (!reusable(t)) break;
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb) {
           const int i = t * SB + sb;
-          if (i < nb) {
+          if (i < whole) {
+            put(i, ahead[sb % AHEAD]);
+            load(i + AHEAD, ahead[sb % AHEAD]);
+          } else if (i < nb) {
+            Raw raw[PER];
 #pragma unroll
-            for (int u = 0; u < PER; ++u) {
-              const int m = row0 + u * rows_step;
-              if (m >= mrows) continue;
-              uint4 out[PARTS];
-              X::stage(next[u], out);
-#pragma unroll
-              for (int q = 0; q < PARTS; ++q)
-                *reinterpret_cast<uint4*>(place(i, m * PARTS + q)) = out[q];
-            }
-            load(i + 1);
+            for (int u = 0; u < PER; ++u)
+              raw[u] = X::load(rows[u] - c * 8 * X::kBytes, (int64_t)i * kBlockK + c * 8,
+                               K - b0 * kBlockK, false);
+            put(i, raw);
           }
         }
         post(t);
@@ -470,7 +482,7 @@ template <int XT, int NC, int UNIT>
 int launch(W4Params p, int* status, cudaStream_t st) {
   auto kernel = dense_w4_tc_kernel<XT, NC, UNIT>;
   using S = Stage<NC, UNIT>;
-  constexpr int PARTS = XRow<XT>::kParts, PER_SM = 1;
+  constexpr int PARTS = XRow<XT>::kParts;
   p.rows = NC / PARTS;
   const int64_t tiles = (p.a.w.N + kTileN - 1) / kTileN;
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
@@ -481,7 +493,7 @@ int launch(W4Params p, int* status, cudaStream_t st) {
   int best = 0;
   int64_t least = INT64_MAX;
   for (int l = 0; l <= 3; ++l) {
-    const int64_t waves = ((tiles * chunks << l) + 148 * PER_SM - 1) / (148 * PER_SM);
+    const int64_t waves = ((tiles * chunks << l) + 148 - 1) / 148;
     const int64_t blocks = (p.kblocks + (1 << l) - 1) >> l;
     const int64_t cost = waves * (blocks + kFixed);
     if (cost < least) {
@@ -489,7 +501,6 @@ int launch(W4Params p, int* status, cudaStream_t st) {
       best = l;
     }
   }
-  if (const char* e = getenv("W4C"); e && atoi(e) >= 0) best = atoi(e);
   const int C = 1 << best;
   p.log_cluster = best;
   const int rows = (int)std::min<int64_t>(p.rows, p.a.M);
