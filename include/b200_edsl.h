@@ -378,13 +378,28 @@ int b200_w4_dequantize(const void* packed, int s_dtype, int has_zeros, int64_t K
  * bf16 or f16. An e4m3 X may have x_scales: one for each row (x_group 0,
  * x_scales[m * ld_x_scales]) or for each x_group (32, 64 or 128) columns, as
  * b200_rms_norm writes them. Products are exact and sums run in f32 (an f32 X
- * keeps all its bits); Y is rounded once. The weights are read once for each
- * 64 rows (f32: 21 rows), so many rows are better served by
- * b200_w4_dequantize and b200_dense_f32. */
+ * keeps all its bits); Y is rounded once. Up to 8 rows (f32: 2) run on
+ * mma.sync, more on tcgen05; the weights are read once for each 128 rows (64
+ * with groups of 32; f32: a third of that), so several hundred rows are better
+ * served by b200_w4_dequantize and b200_dense_f32. The first call on a device
+ * (or b200_w4_pack) makes the runtime's state there; make it before any stream
+ * capture. */
 int b200_dense_w4(const void* X, int64_t ldx, int x_dtype, const float* x_scales,
                   int64_t ld_x_scales, int x_group, const void* packed, int s_dtype, int has_zeros,
                   int group, const void* b, int b_dtype, void* Y, int64_t ldy, int y_dtype,
                   int64_t M, int64_t N, int64_t K, int act, float alpha, void* stream);
+
+/* 4-bit weights of a host matrix, kept on each GPU like b200_weights_register
+ * keeps f32 ones: b200_weights_register_w4 declares the f32 W[K,N] at host
+ * address W unchanged until it is registered with another version (or shape
+ * or group) or released; b200_weights_w4 gives its packed form on the current
+ * device (b200_w4_quantize with f32 scales, no zeros), made at first use;
+ * b200_weights_release_w4 frees it on every GPU. Neither registering anew nor
+ * releasing may overlap a call that uses the weights on another thread. */
+int b200_weights_register_w4(const float* W, int64_t ldw, int64_t K, int64_t N, int group,
+                             uint64_t version);
+int b200_weights_w4(const float* W, const void** packed);
+int b200_weights_release_w4(const float* W);
 
 /* Over rows of logits [T,V] (f32, bf16 or f16) and p = softmax(row):
  *   logprobs[t] = log p[tokens[t]]        (tokens and logprobs, or both NULL);

@@ -503,6 +503,29 @@ int weights_ready(DeviceCtx* c, const float* Whost, WeightEntry* e, bool mn, Pre
   return kOk;
 }
 
+// Weights kept in 4 bits (b200_weights_register_w4): a registered host W[K, N]
+// whose packed form (w4_pack, f32 scales) is made on each device at first use.
+struct W4Entry {
+  W4Layout layout;
+  int64_t ldw = 0;
+  uint64_t version = 0;
+  DevBuf packed[64];
+};
+std::map<const float*, std::unique_ptr<W4Entry>> g_w4;  // by host address; under g_w_mu
+
+// Frees an entry's copies, after the work that may still read them.
+void drop_w4_copies(W4Entry* e) {
+  int prev = 0;
+  const bool have_prev = cudaGetDevice(&prev) == cudaSuccess;
+  for (int d = 0; d < 64; ++d)
+    if (e->packed[d].p) {
+      cudaSetDevice(d);
+      cudaDeviceSynchronize();
+      e->packed[d].release();
+    }
+  if (have_prev) cudaSetDevice(prev);
+}
+
 void release_weight_copy(WeightCopy& d) {
   d.w.release();
   d.lo_mn.release();
@@ -1046,6 +1069,7 @@ int b200_release(void) {
     {
       std::lock_guard<std::mutex> g(g_w_mu);
       for (auto& kv : g_weights) release_weight_copy(kv.second->dev[d]);
+      for (auto& kv : g_w4) kv.second->packed[d].release();
     }
     std::vector<StreamScratch*> entries;
     {
@@ -1108,6 +1132,81 @@ int b200_weights_release(const float* W) {
   }
   g_weights.erase(it);
   if (have_prev) cudaSetDevice(prev);
+  return succeed();
+}
+
+int b200_weights_register_w4(const float* W, int64_t ldw, int64_t K, int64_t N, int group,
+                             uint64_t version) {
+  if (!W || K <= 0 || N <= 0 || ldw < N)
+    return fail(kErrInvalidArg, "weights: non-null W, K > 0, N > 0 and ldw >= N are required");
+  if (b200_w4_bytes(K, N, group, kF32, 0) < 0) return t_status;
+  std::lock_guard<std::mutex> g(g_w_mu);
+  auto& slot = g_w4[W];
+  if (slot && slot->ldw == ldw && slot->layout.K == K && slot->layout.N == N &&
+      slot->layout.group == group && slot->version == version)
+    return succeed();  // unchanged: keep the packed copies
+  if (slot) drop_w4_copies(slot.get());
+  else slot.reset(new W4Entry);
+  slot->layout.K = K;
+  slot->layout.N = N;
+  slot->layout.group = group;
+  slot->layout.s_dtype = kF32;
+  slot->layout.has_zeros = false;
+  slot->ldw = ldw;
+  slot->version = version;
+  return succeed();
+}
+
+int b200_weights_release_w4(const float* W) {
+  std::lock_guard<std::mutex> g(g_w_mu);
+  auto it = g_w4.find(W);
+  if (it == g_w4.end()) return fail(kErrInvalidArg, "weights: W is not registered");
+  drop_w4_copies(it->second.get());
+  g_w4.erase(it);
+  return succeed();
+}
+
+int b200_weights_w4(const float* W, const void** packed) {
+  if (!W || !packed) return fail(kErrInvalidArg, "weights: null argument");
+  *packed = nullptr;
+  {
+    std::lock_guard<std::mutex> g(g_w_mu);
+    if (!g_w4.count(W)) return fail(kErrInvalidArg, "weights: W is not registered");
+  }
+  DeviceCtx* c = nullptr;
+  int rc = current_ctx(&c);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lk(c->mu);  // the staging buffers of h2d_rows
+  std::lock_guard<std::mutex> g(g_w_mu);
+  auto it = g_w4.find(W);
+  if (it == g_w4.end()) return fail(kErrInvalidArg, "weights: W is not registered");
+  W4Entry* e = it->second.get();
+  const W4Layout& w = e->layout;
+  DevBuf& to = e->packed[c->dev];
+  if (!to.p) {
+    struct Temporary : DevBuf {
+      ~Temporary() { release(); }
+    } f32, codes, scales;
+    DevBuf made;
+    B200_CUDA(f32.reserve((size_t)w.K * w.N * 4), "alloc registered W");
+    B200_CUDA(codes.reserve((size_t)w.K * w.N), "alloc registered W codes");
+    B200_CUDA(scales.reserve((size_t)w.groups() * w.N * 4), "alloc registered W scales");
+    if ((rc = h2d_rows(c, f32.p, w.N * 4, W, e->ldw * 4, w.N * 4, w.K, c->s_comp))) return rc;
+    B200_CUDA(made.reserve((size_t)w.bytes()), "alloc registered W in 4 bits");
+    rc = w4_quantize(static_cast<float*>(f32.p), w.N, w.K, w.N, w.group,
+                     static_cast<uint8_t*>(codes.p), w.N, scales.p, w.N, kF32, c->s_comp);
+    if (rc == kOk)
+      rc = w4_pack(static_cast<uint8_t*>(codes.p), w.N, scales.p, w.N, nullptr, 0, w, made.p,
+                   c->s_comp);
+    const cudaError_t sync = cudaStreamSynchronize(c->s_comp);
+    if (rc || sync != cudaSuccess) {
+      made.release();
+      return rc ? fail(rc, std::string("4 bits of registered W: ") + launch_error_text())
+                : fail_cuda(sync, "sync");
+    }
+    to = made;
+  }
+  *packed = to.p;
   return succeed();
 }
 

@@ -17,7 +17,7 @@ from .ast import (ADD, DIV, MUL, SUB, BinaryOp, Constant, LinalgActivation, Lina
                   LinalgMatmul, Parameter, Value)
 from .functions import MLFunction, ml_function
 from .ops import (If, add, div, dot, eq, ge, gt, le, leaky_relu, lt, matmul, mul, ne, reduce,
-                  relu, sub, tensor_max, tensor_min, tensor_sum)
+                  relu, rms_norm, sub, tensor_max, tensor_min, tensor_sum, token_logprobs)
 from .ast import CompareOp, IfOp, LinalgDot, LinalgReduce, to_value
 from .types import DYN, Tensor, TensorType, ScalarType, f32, i1, i32
 
@@ -36,7 +36,7 @@ __all__ = [
     "ml_function", "MLFunction",
     "i32", "f32", "i1", "DYN", "Tensor", "TensorType", "ScalarType",
     "add", "sub", "mul", "div", "matmul", "relu", "leaky_relu",
-    "dot", "reduce", "tensor_sum", "tensor_max", "tensor_min", "If",
+    "rms_norm", "token_logprobs", "dot", "reduce", "tensor_sum", "tensor_max", "tensor_min", "If",
     "lt", "le", "gt", "ge", "eq", "ne", "to_value", "CompareOp", "IfOp", "LinalgDot",
     "LinalgReduce",
     "ADD", "SUB", "MUL", "DIV",

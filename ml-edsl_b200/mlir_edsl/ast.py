@@ -264,6 +264,60 @@ class LinalgActivation(Value):
         return "relu" if self.act_type == RELU else f"leaky_relu(alpha={self.alpha})"
 
 
+class RmsNorm(Value):
+    """Root-mean-square norm of the rows of a 2-D f32 tensor:
+    h / sqrt(mean(h^2) + eps) * weight with h = input (+ residual)."""
+
+    def __init__(self, input: Value, weight: Value = None, residual: Value = None,
+                 eps: float = 1e-6):
+        super().__init__()
+        self.input, self.weight, self.residual, self.eps = input, weight, residual, float(eps)
+        it = input.infer_type()
+        if not isinstance(it, TensorType) or it.ndim != 2 or not it.is_float():
+            raise TypeError(f"rms_norm: input must be a 2D f32 tensor, got {it}")
+        if weight is not None:
+            wt = weight.infer_type()
+            if not isinstance(wt, TensorType) or wt.ndim != 1 or not wt.is_float():
+                raise TypeError(f"rms_norm: weight must be a 1D f32 tensor, got {wt}")
+            if -1 not in (wt.shape[0], it.shape[1]) and wt.shape[0] != it.shape[1]:
+                raise TypeError(f"rms_norm: weight must have the input's columns, got {it.shape} "
+                                f"and {wt.shape}")
+        if residual is not None and residual.infer_type() != it:
+            raise TypeError(f"rms_norm: residual must have the input's type {it}, got "
+                            f"{residual.infer_type()}")
+        if not 0.0 < self.eps < float("inf"):
+            raise ValueError(f"rms_norm: eps must be positive and finite, got {eps}")
+        self._out_type = it
+
+    def infer_type(self):
+        return self._out_type
+
+    def get_children(self):
+        return [v for v in (self.input, self.weight, self.residual) if v is not None]
+
+
+class TokenLogprobs(Value):
+    """log softmax of each row of a 2-D f32 tensor at the row's i32 token."""
+
+    def __init__(self, logits: Value, tokens: Value):
+        super().__init__()
+        self.logits, self.tokens = logits, tokens
+        lt, tt = logits.infer_type(), tokens.infer_type()
+        if not isinstance(lt, TensorType) or lt.ndim != 2 or not lt.is_float():
+            raise TypeError(f"token_logprobs: logits must be a 2D f32 tensor, got {lt}")
+        if not isinstance(tt, TensorType) or tt.ndim != 1 or not tt.is_integer():
+            raise TypeError(f"token_logprobs: tokens must be a 1D i32 tensor, got {tt}")
+        if -1 not in (lt.shape[0], tt.shape[0]) and lt.shape[0] != tt.shape[0]:
+            raise TypeError(f"token_logprobs: one token a row, got {lt.shape} and {tt.shape}")
+        self._out_type = TensorType((lt.shape[0],), lt.element_type)
+
+    def infer_type(self):
+        return self._out_type
+
+    def get_children(self):
+        return [self.logits, self.tokens]
+
+
 class BinaryOp(Value):
     """Scalar arithmetic between two scalar values (kept for operator
     completeness; the b200 target only lowers tensor patterns)."""

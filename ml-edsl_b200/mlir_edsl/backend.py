@@ -82,17 +82,44 @@ _DEFAULT_INIT = {0: 0.0, 2: float("-inf"), 3: float("inf")}
 # that its memory cannot be reused by another array while registered.
 _WEIGHTS: Dict[int, Tuple[np.ndarray, int]] = {}
 
+# Arrays registered with 4 bits: data address -> (array, version, group).
+_WEIGHTS_4BIT: Dict[int, Tuple[np.ndarray, int, int]] = {}
 
-def register_weights(W: np.ndarray, version: int = 0) -> None:
+# Rows up to which a function runs on 4-bit weights as they are; more rows use
+# their f32 values with the f32 GEMM (K 4096, N 11008, f32 rows: 188 us against
+# 275 at 128 rows, 326 against 318 at 256, 581 against 378 at 512).
+W4_ROWS = 256
+
+
+def register_weights(W: np.ndarray, version: int = 0, *, bits: int = 32,
+                     group: int = 128) -> None:
     """Declares the 2-D f32 array W unchanged until it is registered again
     with another version or released: the device copy and tf32 split of W
     are then kept on every GPU that runs a function taking it, instead of
     being copied and split in every call (b200_weights_register). Modifying
-    W in place without re-registering it leaves later calls on stale data."""
+    W in place without re-registering it leaves later calls on stale data.
+
+    bits=4 keeps W in 4 bits instead, with a scale for each `group` (32 or a
+    multiple of 64) rows of each column (b200_weights_register_w4): functions
+    that multiply by W then do so by its 4-bit values."""
     if not isinstance(W, np.ndarray) or W.dtype != np.float32 or W.ndim != 2:
         raise TypeError("register_weights takes a 2-D float32 ndarray")
     if not W.flags["C_CONTIGUOUS"]:
         raise ValueError("register_weights takes a C-contiguous array")
+    if bits not in (4, 32):
+        raise ValueError(f"register_weights keeps 4 or 32 bits, got {bits}")
+    if bits == 4:
+        if group != 32 and (group <= 0 or group % 64):
+            raise ValueError(f"group must be 32 or a multiple of 64, got {group}")
+        if W.ctypes.data in _WEIGHTS:
+            release_weights(W)
+        _native.check(_native.lib().b200_weights_register_w4(
+            ctypes.c_void_p(W.ctypes.data), W.shape[1], W.shape[0], W.shape[1], int(group),
+            int(version)))
+        _WEIGHTS_4BIT[W.ctypes.data] = (W, int(version), int(group))
+        return
+    if W.ctypes.data in _WEIGHTS_4BIT:
+        release_weights(W)
     _native.check(_native.lib().b200_weights_register(
         ctypes.c_void_p(W.ctypes.data), W.shape[1], W.shape[0], W.shape[1], int(version)))
     _WEIGHTS[W.ctypes.data] = (W, int(version))
@@ -100,6 +127,10 @@ def register_weights(W: np.ndarray, version: int = 0) -> None:
 
 def release_weights(W: np.ndarray) -> None:
     """Frees the device copies of a registered array and forgets it."""
+    if W.ctypes.data in _WEIGHTS_4BIT:
+        del _WEIGHTS_4BIT[W.ctypes.data]
+        _native.check(_native.lib().b200_weights_release_w4(ctypes.c_void_p(W.ctypes.data)))
+        return
     if W.ctypes.data not in _WEIGHTS:
         raise ValueError("array is not registered")
     del _WEIGHTS[W.ctypes.data]
@@ -109,6 +140,14 @@ def release_weights(W: np.ndarray) -> None:
 def _registered(a: np.ndarray) -> bool:
     held = _WEIGHTS.get(a.ctypes.data)
     return held is not None and held[0].shape == a.shape and a.dtype == np.float32
+
+
+def _group_4bit(a):
+    """The group of an array that is registered with 4 bits, else None."""
+    if not isinstance(a, np.ndarray) or a.dtype != np.float32:
+        return None
+    held = _WEIGHTS_4BIT.get(a.ctypes.data)
+    return held[2] if held is not None and held[0].shape == a.shape else None
 
 
 def _to_python(v):
@@ -199,6 +238,8 @@ class B200Backend:
                 if step.shape == ():
                     return self._run_scalar_host(step, values)
                 sym = _memref_symbol(step)
+                if step.op == "gemm_f32" and _group_4bit(values[step.inputs[1].index]):
+                    sym = None  # the device path knows 4-bit weights
                 if sym is not None:
                     return self._run_memref(sym, plan, param_types, values)
             return self._run_device(plan, param_types, values)
@@ -267,8 +308,13 @@ class B200Backend:
 
         try:
             dparams = {}
-            needed = {r.index for s in plan.steps for r in s.inputs
-                      if r.kind == "param" and s.op != "scalar_op"}
+            # f32 GEMMs by weights registered with 4 bits: step -> group; those
+            # weights need no f32 copy
+            w4 = {i: _group_4bit(arrays[s.inputs[1].index]) for i, s in enumerate(plan.steps)
+                  if s.op == "gemm_f32" and s.inputs[1].kind == "param"}
+            needed = {r.index for i, s in enumerate(plan.steps) for j, r in enumerate(s.inputs)
+                      if r.kind == "param" and s.op != "scalar_op"
+                      and not (j == 1 and w4.get(i))}
             for i in sorted(needed):
                 a = arrays[i]
                 if isinstance(a, np.ndarray) and a.ndim == 2 and _registered(a):
@@ -285,8 +331,8 @@ class B200Backend:
             # f32 GEMM outputs that a later f32 GEMM reads as its A operand:
             # their epilogue also writes the tf32 lo part, so that the next
             # layer does not split them again (b200_dense_f32_chain)
-            feeds_a = {st.inputs[0].index for st in plan.steps
-                       if st.op == "gemm_f32" and st.inputs[0].kind == "step"}
+            feeds_a = {st.inputs[0].index for i, st in enumerate(plan.steps)
+                       if st.op == "gemm_f32" and st.inputs[0].kind == "step" and not w4.get(i)}
             lo_of = {}
 
             def dref(r: Ref):
@@ -294,6 +340,12 @@ class B200Backend:
 
             def shape_of(r: Ref):
                 return arrays[r.index].shape if r.kind == "param" else plan.steps[r.index].shape
+
+            def packed_w4(r: Ref):
+                p = ctypes.c_void_p()
+                _native.check(L.b200_weights_w4(ctypes.c_void_p(arrays[r.index].ctypes.data),
+                                                ctypes.byref(p)))
+                return p
 
             for s in plan.steps:
                 nelem = int(np.prod(s.shape))  # 1 for scalar results
@@ -304,7 +356,19 @@ class B200Backend:
                     M, K = shape_of(a)
                     N = shape_of(b)[1]
                     bias = dref(s.inputs[2]) if s.has_bias else None
-                    if s.op == "gemm_f32":
+                    group = w4.get(len(douts) - 1)
+                    if group and M <= W4_ROWS:
+                        _native.check(L.b200_dense_w4(
+                            dref(a), K, _native.F32, None, 0, 0, packed_w4(b), _native.F32, 0,
+                            group, bias, _native.F32, out, N, _native.F32, M, N, K, s.act, s.alpha,
+                            None))
+                    elif group:
+                        w = dmalloc(K * N * 4)
+                        _native.check(L.b200_w4_dequantize(packed_w4(b), _native.F32, 0, K, N,
+                                                           group, w, N, None))
+                        _native.check(L.b200_dense_f32(dref(a), K, w, N, bias, out, N, M, N, K,
+                                                       s.act, s.alpha, None))
+                    elif s.op == "gemm_f32":
                         me = len(douts) - 1
                         # the next layer reads this lo part with its split pitch
                         ldylo = _native.split_pitch(N)
@@ -336,6 +400,19 @@ class B200Backend:
                     M, N = s.shape
                     _native.check(L.b200_bias_add_i32(dref(s.inputs[0]), N, dref(s.inputs[1]),
                                                       out, N, M, N, None))
+                elif s.op == "rms_norm_f32":
+                    M, N = s.shape
+                    rest = [dref(r) for r in s.inputs[1:]]
+                    w = rest.pop(0) if s.has_bias else None
+                    r = rest.pop(0) if s.has_residual else None
+                    _native.check(L.b200_rms_norm(dref(s.inputs[0]), N, r, N, _native.F32, w,
+                                                  _native.F32, s.eps, None, N, out, N, _native.F32,
+                                                  None, 0, 0, M, N, None))
+                elif s.op == "token_logprobs_f32":
+                    T, V = shape_of(s.inputs[0])
+                    _native.check(L.b200_token_logprobs(dref(s.inputs[0]), V, _native.F32, T, V,
+                                                        dref(s.inputs[1]), out, None, 0, None, None,
+                                                        None))
                 elif s.op in ("dot_f32", "dot_i32"):
                     a, b = s.inputs
                     n = int(np.prod(shape_of(a)))

@@ -12,6 +12,7 @@ one fused kernel step:
   X + b, relu(X + b), relu(X), leaky(X)  -> bias_act (HBM-bound elementwise)
   dot(a, b), tensor_sum/max/min, reduce  -> dot / reduce (HBM-bound, two-pass)
   scalar arithmetic on those results     -> a host step after the device work
+  rms_norm, token_logprobs               -> their own steps (HBM-bound, one launch)
 
 A producer is folded into its consumer only when the consumer is its sole
 use (SSA values used twice stay materialised). Chains of layers become
@@ -23,7 +24,7 @@ from typing import Dict, List, Optional, Tuple
 
 from .ast import (ADD, MUL, LEAKY_RELU, RELU, TENSOR_BIAS_LEFT, TENSOR_BIAS_RIGHT, BinaryOp,
                   CompareOp, Constant, IfOp, LinalgActivation, LinalgBinaryOp, LinalgDot,
-                  LinalgMatmul, LinalgReduce, OP_NAMES, Parameter, Value)
+                  LinalgMatmul, LinalgReduce, OP_NAMES, Parameter, RmsNorm, TokenLogprobs, Value)
 from .types import ScalarType, TensorType
 
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU = 0, 1, 2
@@ -41,7 +42,8 @@ class Ref:
 @dataclass
 class Step:
     op: str                 # "gemm_f32" | "gemm_i32" | "bias_act_f32" | "bias_add_i32" |
-                            # "dot_{f32,i32}" | "reduce_{f32,i32}" | "scalar_op" (host)
+                            # "dot_{f32,i32}" | "reduce_{f32,i32}" | "scalar_op" (host) |
+                            # "rms_norm_f32" | "token_logprobs_f32"
     inputs: List[Ref]       # gemm: [A, B(, bias)]; bias_act: [X(, bias)]; dot: [a, b]
     shape: Tuple[int, ...]  # output shape (() for scalars)
     dtype: str              # "f32" | "i32"
@@ -51,6 +53,8 @@ class Step:
     red_op: int = REDUCE_SUM   # reduce: the fold
     init: float = 0.0          # reduce: initial accumulator
     scalar_op: int = ADD       # scalar_op: ADD/SUB/MUL/DIV
+    has_residual: bool = False  # rms_norm: inputs are x, then weight, then residual
+    eps: float = 0.0
 
     def describe(self, names) -> str:
         args = ", ".join(names(r) for r in self.inputs)
@@ -59,6 +63,8 @@ class Step:
                     f"-> {self.dtype}")
         if self.op == "scalar_op":
             return f"host {OP_NAMES[self.scalar_op]}({args}) -> {self.dtype}"
+        if self.op == "rms_norm_f32":
+            return f"{self.op}({args}, eps={self.eps}) -> {self.dtype}{list(self.shape)}"
         act = {ACT_NONE: "", ACT_RELU: ", act=relu",
                ACT_LEAKY_RELU: f", act=leaky_relu({self.alpha})"}[self.act]
         return f"{self.op}({args}{act}) -> {self.dtype}{list(self.shape)}"
@@ -197,6 +203,13 @@ def lower(root: Value, param_names: List[str]) -> Plan:
                 s.act, s.alpha = act, node.alpha
                 return src
             return emit(Step("bias_act_f32", [src], t.shape, dt, act=act, alpha=node.alpha))
+        if isinstance(node, RmsNorm):
+            return emit(Step("rms_norm_f32", [visit(c) for c in node.get_children()],
+                             node.infer_type().shape, "f32", has_bias=node.weight is not None,
+                             has_residual=node.residual is not None, eps=node.eps))
+        if isinstance(node, TokenLogprobs):
+            return emit(Step("token_logprobs_f32", [visit(node.logits), visit(node.tokens)],
+                             node.infer_type().shape, "f32"))
         if isinstance(node, LinalgDot):
             a, b = visit(node.lhs), visit(node.rhs)
             dt = _dtype(node.infer_type())

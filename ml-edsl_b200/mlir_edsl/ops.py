@@ -27,6 +27,21 @@ def leaky_relu(arr: Value, alpha: float = 0.01) -> LinalgActivation:
     return LinalgActivation(arr, LEAKY_RELU, float(alpha))
 
 
+def rms_norm(arr: Value, weight: Value = None, residual: Value = None, eps: float = 1e-6):
+    """h / sqrt(mean(h^2) + eps) * weight over the rows of a 2-D f32 tensor,
+    h = arr (+ residual). No counterpart in the reference."""
+    from .ast import RmsNorm
+    return RmsNorm(arr, weight, residual, eps)
+
+
+def token_logprobs(logits: Value, tokens: Value):
+    """Log probability of each row's token ([T] i32) under the softmax of the
+    row's logits ([T, V] f32): 0 for a negative token (a padded row), NaN for
+    one past V. No counterpart in the reference."""
+    from .ast import TokenLogprobs
+    return TokenLogprobs(logits, tokens)
+
+
 def _dispatch_binary_op(op: int, left: Value, right: Value):
     lt, rt = left.infer_type(), right.infer_type()
     if isinstance(lt, TensorType) or isinstance(rt, TensorType):

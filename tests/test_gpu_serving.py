@@ -529,3 +529,89 @@ def test_gradients_are_refused(cuda):
         serving.rms_norm(x)
     with pytest.raises(ValueError, match="no backward pass"):
         serving.token_logprobs(x)
+
+
+# ------------------------------------------------------------------- frontend
+
+@pytest.mark.parametrize("M", [1, 7, 300])
+@pytest.mark.parametrize("bits,group", [(32, 128), (4, 32), (4, 128)])
+def test_frontend_network(cuda, M, bits, group):
+    """norm -> dense layer -> dense layer -> log probabilities as one traced
+    function, with f32 weights and with weights registered in 4 bits. Errors
+    are carried through: of the norm, then of each layer 2^-18 of the sum of
+    absolute products (3xTF32 drops 2^-20 of it, the 4-bit layer 2^-19), then
+    twice the row's largest."""
+    import numpy as np
+    from mlir_edsl import (Tensor, f32, get_backend, i32, ml_function, register_weights,
+                           release_weights, relu, rms_norm, token_logprobs)
+    K, H, V = 200, 320, 517
+    rng = np.random.default_rng(M)
+    X, R = (rng.standard_normal((M, K)).astype(np.float32) for _ in range(2))
+    w = (1 + 0.1 * rng.standard_normal(K)).astype(np.float32)
+    W1 = (rng.standard_normal((K, H)) / K ** 0.5).astype(np.float32)
+    b1 = rng.standard_normal(H).astype(np.float32)
+    W2 = (rng.standard_normal((H, V)) / H ** 0.5).astype(np.float32)
+    tokens = rng.integers(0, V, M).astype(np.int32)
+    tokens[-1] = -1 if M > 1 else tokens[-1]
+
+    @ml_function(target="b200")
+    def net(X: Tensor[f32, M, K], R: Tensor[f32, M, K], w: Tensor[f32, K], W1: Tensor[f32, K, H],
+            b1: Tensor[f32, H], W2: Tensor[f32, H, V], tokens: Tensor[i32, M]) -> Tensor[f32, M]:
+        return token_logprobs(relu(rms_norm(X, w, R) @ W1 + b1) @ W2, tokens)
+
+    D1, D2 = torch.from_numpy(W1).to(cuda), torch.from_numpy(W2).to(cuda)
+    if bits == 4:
+        D1, D2 = (serving.quantize_w4(d, group=group).dequantize() for d in (D1, D2))
+        register_weights(W1, bits=4, group=group)
+        register_weights(W2, bits=4, group=group)
+    try:
+        got = net(X, R, w, W1, b1, W2, tokens)
+        again = net(X, R, w, W1, b1, W2, tokens)
+        if bits == 4 and M <= 256:
+            assert get_backend().last_launches == 4  # one kernel a step, nothing packed again
+    finally:
+        if bits == 4:
+            release_weights(W1)
+            release_weights(W2)
+    assert got.shape == (M,) and np.array_equal(got, again)
+    D1, D2 = D1.double(), D2.double()
+    x, r, bd = (torch.from_numpy(a).to(cuda) for a in (X, R, b1))
+    y = norm_formula(x, torch.from_numpy(w).to(cuda), r, 1e-6)
+    err = NORM_F32 * y.abs()
+    a = y @ D1 + bd.double()
+    err = err @ D1.abs() + 2.0 ** -18 * (y.abs() @ D1.abs()) + 2.0 ** -23 * a.abs()
+    a = a.clamp(min=0)
+    logits = a @ D2
+    err = err @ D2.abs() + 2.0 ** -18 * (a.abs() @ D2.abs())
+    t = torch.from_numpy(tokens).to(cuda).long()
+    want = torch.log_softmax(logits, 1).gather(1, t.clamp(min=0)[:, None])[:, 0]
+    want = torch.where(t < 0, torch.zeros_like(want), want)
+    room = 2 * err.amax(1) + 2.0 ** -16
+    diff = (torch.from_numpy(got).to(cuda).double() - want).abs()
+    assert (diff <= room).all(), (diff / room).max()
+
+
+def test_frontend_4_bit_weights_follow_versions(cuda):
+    import numpy as np
+    from mlir_edsl import Tensor, f32, ml_function, register_weights, release_weights
+    W = np.ones((64, 64), np.float32)
+    X = np.ones((2, 64), np.float32)
+
+    @ml_function(target="b200")
+    def f(X: Tensor[f32, 2, 64], W: Tensor[f32, 64, 64]) -> Tensor[f32, 2, 64]:
+        return X @ W
+
+    register_weights(W, 1, bits=4, group=64)
+    try:
+        np.testing.assert_allclose(f(X, W), 64, rtol=2.0 ** -20)
+        W *= 2
+        np.testing.assert_allclose(f(X, W), 64, rtol=2.0 ** -20)  # the documented contract
+        register_weights(W, 2, bits=4, group=64)
+        np.testing.assert_allclose(f(X, W), 128, rtol=2.0 ** -20)
+        _native.check(_native.lib().b200_release())  # copies are made again
+        np.testing.assert_allclose(f(X, W), 128, rtol=2.0 ** -20)
+        register_weights(W, 2)  # back to 32 bits
+        np.testing.assert_array_equal(f(X, W), 128)
+    finally:
+        release_weights(W)
+    np.testing.assert_array_equal(f(X, W), 128)

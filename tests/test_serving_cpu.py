@@ -173,3 +173,72 @@ def test_rows_of_tensors():
               torch.zeros(1, 2, 6).expand(4, 2, 6)):
         with pytest.raises(ValueError):
             rows(t)
+
+
+# ------------------------------------------------------------------- frontend
+def _plan(fn):
+    from mlir_edsl.functions import FunctionSignature, validate_function_body
+    from mlir_edsl.lowering import lower
+    sig = FunctionSignature.from_callable(fn)
+    ast, _ = validate_function_body(fn, sig)
+    return lower(ast, sig.param_names)
+
+
+def test_frontend_steps():
+    from mlir_edsl import Tensor, f32, i32, relu, rms_norm, token_logprobs
+
+    def net(X: Tensor[f32, 3, 8], R: Tensor[f32, 3, 8], w: Tensor[f32, 8], W: Tensor[f32, 8, 5],
+            b: Tensor[f32, 5], t: Tensor[i32, 3]) -> Tensor[f32, 3]:
+        return token_logprobs(relu(rms_norm(X, w, R, eps=1e-5) @ W + b), t)
+    plan = _plan(net)
+    assert [s.op for s in plan.steps] == ["rms_norm_f32", "gemm_f32", "token_logprobs_f32"]
+    norm, gemm, score = plan.steps
+    assert [plan.params[r.index] for r in norm.inputs] == ["X", "w", "R"]
+    assert norm.has_bias and norm.has_residual and norm.eps == 1e-5 and norm.shape == (3, 8)
+    assert gemm.has_bias and score.shape == (3,)
+    assert "rms_norm_f32(X, w, R, eps=1e-05) -> f32[3, 8]" in plan.describe()
+
+    def bare(X: Tensor[f32, 3, 8], R: Tensor[f32, 3, 8]) -> Tensor[f32, 3, 8]:
+        return rms_norm(X, residual=R)
+    step = _plan(bare).steps[0]
+    assert not step.has_bias and step.has_residual and step.eps == 1e-6
+
+
+def test_frontend_refusals():
+    from mlir_edsl import Tensor, f32, i32, rms_norm, token_logprobs
+    from mlir_edsl.ast import Parameter
+    P = lambda t: Parameter("p", t)
+    x = P(Tensor[f32, 3, 8])
+    for args, text in (((P(Tensor[f32, 8]),), "2D f32"), ((P(Tensor[i32, 3, 8]),), "2D f32"),
+                       ((x, P(Tensor[f32, 7])), "columns"), ((x, P(Tensor[i32, 8])), "1D f32"),
+                       ((x, None, P(Tensor[f32, 3, 7])), "residual")):
+        with pytest.raises(TypeError, match=text):
+            rms_norm(*args)
+    with pytest.raises(ValueError, match="eps"):
+        rms_norm(x, eps=0.0)
+    for args, text in (((P(Tensor[i32, 3, 8]), P(Tensor[i32, 3])), "logits"),
+                       ((x, P(Tensor[f32, 3])), "tokens"), ((x, P(Tensor[i32, 4])), "one token")):
+        with pytest.raises(TypeError, match=text):
+            token_logprobs(*args)
+
+
+def test_register_weights_with_4_bits_refusals():
+    import numpy as np
+    from mlir_edsl import register_weights, release_weights
+    W = np.ones((64, 8), np.float32)
+    with pytest.raises(ValueError, match="4 or 32"):
+        register_weights(W, bits=8)
+    with pytest.raises(ValueError, match="group"):
+        register_weights(W, bits=4, group=48)
+    with pytest.raises(ValueError, match="not registered"):
+        release_weights(W)
+    register_weights(W, bits=4, group=32)  # nothing is packed before its first use
+    register_weights(W, bits=4, group=64)
+    release_weights(W)
+    L = _native.lib()
+    at = ctypes.c_void_p(W.ctypes.data)
+    assert L.b200_weights_release_w4(at) == INVALID
+    assert L.b200_weights_register_w4(at, 8, 64, 8, 33, 0) == INVALID
+    assert L.b200_weights_register_w4(at, 7, 64, 8, 32, 0) == INVALID
+    out = ctypes.c_void_p()
+    assert L.b200_weights_w4(at, ctypes.byref(out)) == INVALID and not out.value
