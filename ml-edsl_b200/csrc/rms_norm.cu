@@ -53,30 +53,37 @@ __device__ __forceinline__ float row_reduce(float v, float* sh) {
   return v;
 }
 
-// Elements [n, n + VEC) of a row as floats, 0 past N.
+// How the rows lie: on 16 bytes; anyhow (element by element); or, rows of an
+// odd length in a buffer that starts on 16 bytes, each with the same cut off
+// 16 bytes in every tensor. A cut row's chunks are those of the memory, so
+// that all but its first and last one are 16-byte accesses (1000x1001 f32
+// without residual: see the launcher).
+enum Rows { kAligned, kAnyhow, kCut };
+
+// Elements [n, n + VEC) of a row as floats, 0 past N (and before 0).
 template <class T, bool AL>
 __device__ __forceinline__ void load_chunk(const T* row, int64_t n, int64_t N, float* f) {
   constexpr int VEC = Chunk<T>::kElems;
-  if (AL && n + VEC <= N) {
+  if (AL && n >= 0 && n + VEC <= N) {
     // an ordinary load: h may be stored over x or over the residual
     unpack(*reinterpret_cast<const uint4*>(row + n), (const T*)nullptr, f);
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = n + i < N ? to_f32(row[n + i]) : 0.0f;
+    for (int i = 0; i < VEC; ++i) f[i] = n + i >= 0 && n + i < N ? to_f32(row[n + i]) : 0.0f;
   }
 }
 
 template <class T, bool AL>
 __device__ __forceinline__ void store_chunk(T* row, int64_t n, int64_t N, const float* f) {
   constexpr int VEC = Chunk<T>::kElems;
-  if (AL && n + VEC <= N) {
+  if (AL && n >= 0 && n + VEC <= N) {
     // streaming: outputs do not push the rows that are still to be read out of
     // L2 (65536x4096 bf16 with residual: 370 -> 357 us; loads gain nothing)
     __stcs(reinterpret_cast<uint4*>(row + n), pack(f, (const T*)nullptr));
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
-      if (n + i < N) row[n + i] = from_f32<T>(f[i]);
+      if (n + i >= 0 && n + i < N) row[n + i] = from_f32<T>(f[i]);
   }
 }
 
@@ -113,7 +120,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t n, int64_t N, 
                                                 __NV_SATFINITE, __NV_E4M3);
     w[i] = a | b << 16;
   }
-  if (AL && n + VEC <= N) {
+  if (AL && n >= 0 && n + VEC <= N) {
     if constexpr (VEC == 8)
       *reinterpret_cast<uint2*>(row + n) = make_uint2(w[0], w[1]);
     else
@@ -121,7 +128,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t n, int64_t N, 
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
-      if (n + i < N) row[n + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+      if (n + i >= 0 && n + i < N) row[n + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
   }
 }
 
@@ -157,12 +164,12 @@ struct RawChunk {
   uint4 v;
   __device__ __forceinline__ void load(const T* row, int64_t n, int64_t N) {
     constexpr int VEC = Chunk<T>::kElems;
-    if (n + VEC <= N) {
+    if (n >= 0 && n + VEC <= N) {
       v = *reinterpret_cast<const uint4*>(row + n);
     } else {
       float f[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) f[i] = n + i < N ? to_f32(row[n + i]) : 0.0f;
+      for (int i = 0; i < VEC; ++i) f[i] = n + i >= 0 && n + i < N ? to_f32(row[n + i]) : 0.0f;
       v = pack(f, (const T*)nullptr);  // the values are T's: nothing is rounded
     }
   }
@@ -184,10 +191,11 @@ struct RawChunk<T, false> {
 // Rows by TPR threads each, E chunks of 16 bytes a thread: chunk e * TPR + t of
 // a row is thread t's e-th. A row is read once and stays in registers; the next
 // row of the CTA is on its way while one is summed, scaled and stored.
-template <class T, int TPR, int E, bool AL>
+template <class T, int TPR, int E, Rows HOW>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
     rms_norm_kernel(const __grid_constant__ RmsNormArgs p) {
   constexpr int VEC = Chunk<T>::kElems;
+  constexpr bool AL = HOW != kAnyhow, WHOLE = HOW == kAligned;
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
   __shared__ float sh[2][3][32];  // in turn, for one row and the next
   const int t = threadIdx.x % TPR;
@@ -196,19 +204,22 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
   pdl_trigger();
   pdl_wait();
   RawChunk<T, AL> xs[E], rs[E];
+  auto cut_of = [&](int64_t m) { return HOW == kCut ? (int)(m * p.ldx & (VEC - 1)) : 0; };
   auto load_row = [&](int64_t m) {
+    const int cut = cut_of(m);
     const T* x = static_cast<const T*>(p.X) + m * p.ldx;
 #pragma unroll
-    for (int e = 0; e < E; ++e) xs[e].load(x, (int64_t)(e * TPR + t) * VEC, p.N);
+    for (int e = 0; e < E; ++e) xs[e].load(x, (int64_t)(e * TPR + t) * VEC - cut, p.N);
     if (p.R) {
       const T* r = static_cast<const T*>(p.R) + m * p.ldr;
 #pragma unroll
-      for (int e = 0; e < E; ++e) rs[e].load(r, (int64_t)(e * TPR + t) * VEC, p.N);
+      for (int e = 0; e < E; ++e) rs[e].load(r, (int64_t)(e * TPR + t) * VEC - cut, p.N);
     }
   };
   if (m < p.M) load_row(m);
   // rows of whole warps: TPR is 32 where a CTA has several
   for (int odd = 0; m < p.M; m += step, odd ^= 1) {
+    const int cut = cut_of(m);
     float h[E][VEC];
 #pragma unroll
     for (int e = 0; e < E; ++e) xs[e].floats(h[e]);
@@ -239,12 +250,12 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
       T* hrow = static_cast<T*>(p.H) + m * p.ldh;
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        store_chunk<T, AL>(hrow, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
+        store_chunk<T, AL>(hrow, (int64_t)(e * TPR + t) * VEC - cut, p.N, h[e]);
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float w[VEC];
-      load_weight<T, AL>(p, (int64_t)(e * TPR + t) * VEC, w);
+      load_weight<T, WHOLE>(p, (int64_t)(e * TPR + t) * VEC - cut, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) h[e][i] = h[e][i] * f.pre * f.inv * w[i];
     }
@@ -252,7 +263,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
       T* y = static_cast<T*>(p.Y) + m * p.ldy;
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        store_chunk<T, AL>(y, (int64_t)(e * TPR + t) * VEC, p.N, h[e]);
+        store_chunk<T, AL>(y, (int64_t)(e * TPR + t) * VEC - cut, p.N, h[e]);
       continue;
     }
     uint8_t* q = static_cast<uint8_t*>(p.Y) + m * p.ldy;
@@ -273,8 +284,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
       if (t == 0) s[0] = scale;
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        store_codes<VEC, AL>(q, (int64_t)(e * TPR + t) * VEC, p.N, h[e], all, scale);
-    } else {
+        store_codes<VEC, AL>(q, (int64_t)(e * TPR + t) * VEC - cut, p.N, h[e], all, scale);
+    } else {  // not of cut rows
       const int lanes = p.group / VEC;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -382,10 +393,10 @@ cudaError_t launch_kernel(Kernel kernel, unsigned grid, int threads, const RmsNo
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <class T, int TPR, int E, bool AL>
+template <class T, int TPR, int E, Rows HOW>
 cudaError_t launch(const RmsNormArgs& p, cudaStream_t st) {
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1, THREADS = TPR < 128 ? 128 : TPR;
-  auto kernel = rms_norm_kernel<T, TPR, E, AL>;
+  auto kernel = rms_norm_kernel<T, TPR, E, HOW>;
   // as many CTAs as fit, each with the rows that fall to it
   static const int per_sm = [&] {
     int n = 0;
@@ -397,17 +408,18 @@ cudaError_t launch(const RmsNormArgs& p, cudaStream_t st) {
   return launch_kernel(kernel, (unsigned)grid, THREADS, p, st);
 }
 
-template <class T, bool AL>
+template <class T, Rows HOW>
 cudaError_t dispatch(const RmsNormArgs& p, cudaStream_t st) {
-  const int64_t c = (p.N + Chunk<T>::kElems - 1) / Chunk<T>::kElems;
-  if (c <= 32) return launch<T, 32, 1, AL>(p, st);
-  if (c <= 128) return launch<T, 32, 4, AL>(p, st);
-  if (c <= 256) return launch<T, 128, 2, AL>(p, st);
-  if (c <= 512) return launch<T, 256, 2, AL>(p, st);
-  if (c <= 1024) return launch<T, 512, 2, AL>(p, st);
-  if (c <= 2048) return launch<T, 512, 4, AL>(p, st);
-  if (c <= 4096) return launch<T, 1024, 4, AL>(p, st);
-  return launch_kernel(rms_norm_long_kernel<T, AL>, (unsigned)p.M, 1024, p, st);
+  constexpr int VEC = Chunk<T>::kElems;
+  const int64_t c = (p.N + (HOW == kCut ? VEC - 1 : 0) + VEC - 1) / VEC;
+  if (c <= 32) return launch<T, 32, 1, HOW>(p, st);
+  if (c <= 128) return launch<T, 32, 4, HOW>(p, st);
+  if (c <= 256) return launch<T, 128, 2, HOW>(p, st);
+  if (c <= 512) return launch<T, 256, 2, HOW>(p, st);
+  if (c <= 1024) return launch<T, 512, 2, HOW>(p, st);
+  if (c <= 2048) return launch<T, 512, 4, HOW>(p, st);
+  if (c <= 4096) return launch<T, 1024, 4, HOW>(p, st);
+  return launch_kernel(rms_norm_long_kernel<T, HOW == kAligned>, (unsigned)p.M, 1024, p, st);
 }
 
 template <class T>
@@ -419,7 +431,14 @@ cudaError_t dispatch_aligned(const RmsNormArgs& p, cudaStream_t st) {
   const bool al = ok(p.X, p.ldx, VEC, 16) && (!p.R || ok(p.R, p.ldr, VEC, 16)) &&
                   (!p.H || ok(p.H, p.ldh, VEC, 16)) && (!p.w || ok(p.w, VEC, VEC, 16)) &&
                   (p.scales ? ok(p.Y, p.ldy, VEC, VEC) : ok(p.Y, p.ldy, VEC, 16));
-  return al ? dispatch<T, true>(p, st) : dispatch<T, false>(p, st);
+  if (al) return dispatch<T, kAligned>(p, st);
+  auto same = [](const void* q, int64_t ld, int64_t ldx, int bytes) {
+    return (reinterpret_cast<uintptr_t>(q) % bytes) == 0 && (ld - ldx) % VEC == 0;
+  };
+  const bool cut = p.group == 0 && same(p.X, p.ldx, p.ldx, 16) &&
+                   (!p.R || same(p.R, p.ldr, p.ldx, 16)) && (!p.H || same(p.H, p.ldh, p.ldx, 16)) &&
+                   same(p.Y, p.ldy, p.ldx, p.scales ? VEC : 16);
+  return cut ? dispatch<T, kCut>(p, st) : dispatch<T, kAnyhow>(p, st);
 }
 
 }  // namespace
