@@ -183,6 +183,7 @@ struct RmsNormArgs {
   float eps;
   int w_f32;
   int group;
+  int group_shift;  // log2 of it
 };
 int rms_norm(const RmsNormArgs& p, int dtype, cudaStream_t st);
 

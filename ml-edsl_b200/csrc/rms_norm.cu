@@ -22,9 +22,9 @@ namespace b200 {
 namespace {
 
 constexpr float kE4M3Max = 448.0f;
-// Below this maximum 448 / max leaves the range of f32 (or nears it): the
-// codes are then divided by the scale instead.
-constexpr float kTinyMax = 1e-30f;
+// Outside these maxima 448 / max leaves the range of f32 or of the fast
+// division.
+constexpr float kTinyMax = 1e-30f, kHugeMax = 1e37f;
 
 struct Sum {
   static __device__ __forceinline__ float id() { return 0.0f; }
@@ -103,14 +103,13 @@ __device__ __forceinline__ void load_weight(const RmsNormArgs& p, int64_t n, flo
   }
 }
 
-// Codes of VEC values with the scale of their row or group.
-template <int VEC, bool AL>
+// Codes of VEC values; factor(i) scales value i into e4m3's range.
+template <int VEC, bool AL, class Factor>
 __device__ __forceinline__ void store_codes(uint8_t* row, int64_t n, int64_t N, const float* y,
-                                            float most, float scale) {
+                                            Factor factor) {
   float c[VEC];
-  const float inv = kE4M3Max / most;
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) c[i] = most > kTinyMax ? y[i] * inv : y[i] / scale;
+  for (int i = 0; i < VEC; ++i) c[i] = factor(i, y[i]);
   uint32_t w[VEC / 4];
 #pragma unroll
   for (int i = 0; i < VEC / 4; ++i) {
@@ -132,10 +131,24 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t n, int64_t N, 
   }
 }
 
-__device__ __forceinline__ float scale_of(float most) {
-  const float s = most / kE4M3Max;
-  return s > 0.0f ? s : 1.0f;  // nothing but zeros (or underflow): codes of y itself
-}
+// The scale of a row or group whose largest absolute value is `most`, and the
+// factors that bring its values into range: 448 / most, with the two units in
+// the last place of the fast division. Where most is too small or too large
+// for that the values are moved by 2^100 first.
+struct Scale {
+  float scale, pre, inv;
+  __device__ __forceinline__ explicit Scale(float most) {
+    const float s = most * (1.0f / kE4M3Max);
+    scale = s > 0.0f ? s : 1.0f;  // nothing but zeros (or underflow): codes of y itself
+    pre = 1.0f;
+    inv = s > 0.0f ? __fdividef(kE4M3Max, most) : 1.0f;
+    if (!(most > kTinyMax && most < kHugeMax) && s > 0.0f) {
+      pre = most < 1.0f ? 1.26765060e30f : 7.88860905e-31f;
+      inv = __fdividef(1.0f, scale * pre);
+    }
+  }
+  __device__ __forceinline__ float operator()(float y) const { return y * pre * inv; }
+};
 
 // The largest of a group's absolute values: the group's lanes are
 // group / VEC consecutive ones.
@@ -198,6 +211,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
   constexpr bool AL = HOW != kAnyhow, WHOLE = HOW == kAligned;
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
   __shared__ float sh[2][3][32];  // in turn, for one row and the next
+  constexpr int kRowGroups = ROWS > 1 ? 33 : 1025;  // of 32 columns
+  __shared__ uint32_t sh_groups[2][HOW == kCut ? ROWS * kRowGroups : 1];
   const int t = threadIdx.x % TPR;
   const int64_t step = (int64_t)gridDim.x * ROWS;
   int64_t m = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
@@ -217,6 +232,10 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
     }
   };
   if (m < p.M) load_row(m);
+  if (HOW == kCut && p.group) {
+    for (int g = threadIdx.x; g < ROWS * kRowGroups; g += blockDim.x) sh_groups[0][g] = 0;
+    __syncthreads();
+  }
   // rows of whole warps: TPR is 32 where a CTA has several
   for (int odd = 0; m < p.M; m += step, odd ^= 1) {
     const int cut = cut_of(m);
@@ -280,20 +299,54 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 #pragma unroll
       for (int e = 0; e < E; ++e) all = fmaxf(all, most[e]);
       all = row_reduce<Max, TPR>(all, sh[odd][2]);
-      const float scale = scale_of(all);
-      if (t == 0) s[0] = scale;
+      const Scale scale(all);
+      if (t == 0) s[0] = scale.scale;
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        store_codes<VEC, AL>(q, (int64_t)(e * TPR + t) * VEC - cut, p.N, h[e], all, scale);
-    } else {  // not of cut rows
+        store_codes<VEC, AL>(q, (int64_t)(e * TPR + t) * VEC - cut, p.N, h[e],
+                             [&](int, float y) { return scale(y); });
+    } else if constexpr (HOW == kCut) {
+      // a chunk's elements lie in up to two groups: maxima in shared memory
+      // (of bits, whose order is that of absolute values)
+      uint32_t* gm = sh_groups[odd] + threadIdx.x / TPR * kRowGroups;
+      uint32_t* next = sh_groups[odd ^ 1] + threadIdx.x / TPR * kRowGroups;
+      const int groups = (int)((p.N + p.group - 1) >> p.group_shift);
+      for (int g = t; g < groups; g += TPR) next[g] = 0;  // the row before has been read
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int64_t n = (int64_t)(e * TPR + t) * VEC - cut;
+        if (n >= p.N) continue;
+        const int g0 = n < 0 ? 0 : (int)(n >> p.group_shift);
+        const int in_first = (int)(((int64_t)(g0 + 1) << p.group_shift) - n);
+        float m0 = 0.0f, m1 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (i < in_first) m0 = fmaxf(m0, fabsf(h[e][i]));
+          else m1 = fmaxf(m1, fabsf(h[e][i]));
+        atomicMax(gm + g0, __float_as_uint(m0));
+        if (in_first < VEC && g0 + 1 < groups) atomicMax(gm + g0 + 1, __float_as_uint(m1));
+      }
+      if (TPR > 32) __syncthreads();
+      else __syncwarp();
+      for (int g = t; g < groups; g += TPR) s[g] = Scale(__uint_as_float(gm[g])).scale;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int64_t n = (int64_t)(e * TPR + t) * VEC - cut;
+        if (n >= p.N) continue;
+        const int g0 = n < 0 ? 0 : (int)(n >> p.group_shift);
+        const int in_first = (int)(((int64_t)(g0 + 1) << p.group_shift) - n);
+        const Scale a(__uint_as_float(gm[g0])), b(__uint_as_float(gm[min(g0 + 1, groups - 1)]));
+        store_codes<VEC, AL>(q, n, p.N, h[e],
+                             [&](int i, float y) { return i < in_first ? a(y) : b(y); });
+      }
+    } else {
       const int lanes = p.group / VEC;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const int64_t n = (int64_t)(e * TPR + t) * VEC;
-        const float gm = group_max(most[e], lanes);
-        const float scale = scale_of(gm);
-        if (t % lanes == 0 && n < p.N) s[n / p.group] = scale;
-        store_codes<VEC, AL>(q, n, p.N, h[e], gm, scale);
+        const Scale scale(group_max(most[e], lanes));
+        if ((t & (lanes - 1)) == 0 && n < p.N) s[n >> p.group_shift] = scale.scale;
+        store_codes<VEC, AL>(q, n, p.N, h[e], [&](int, float y) { return scale(y); });
       }
     }
   }
@@ -337,7 +390,7 @@ __global__ void __launch_bounds__(1024)
   const float ss = squares(1.0f, sh[0]);
   const Factor f =
       factor(ss, (float)p.N, p.eps, [&](float c) { return squares(c, sh[1]); });
-  float all = 0.0f, scale = 0.0f;
+  float all = 0.0f;
   if (p.scales && p.group == 0) {
     for (int64_t j = t; j < chunks; j += TPR) {
       float h[VEC], w[VEC];
@@ -347,8 +400,7 @@ __global__ void __launch_bounds__(1024)
       for (int i = 0; i < VEC; ++i) all = fmaxf(all, fabsf(h[i] * f.pre * f.inv * w[i]));
     }
     all = row_reduce<Max, TPR>(all, sh[2]);
-    scale = scale_of(all);
-    if (t == 0) p.scales[m * p.lds] = scale;
+    if (t == 0) p.scales[m * p.lds] = Scale(all).scale;
   }
   // whole warps take part in every step: a group's lanes exchange their maxima
   for (int64_t j0 = 0; j0 < chunks; j0 += TPR) {
@@ -363,16 +415,17 @@ __global__ void __launch_bounds__(1024)
       store_chunk<T, AL>(static_cast<T*>(p.Y) + m * p.ldy, n, p.N, h);
       continue;
     }
-    float most = all, s = scale;
+    float most = all;
     if (p.group) {
       most = 0.0f;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) most = fmaxf(most, fabsf(h[i]));
       most = group_max(most, p.group / VEC);
-      s = scale_of(most);
-      if (n % p.group == 0 && n < p.N) p.scales[m * p.lds + n / p.group] = s;
     }
-    store_codes<VEC, AL>(static_cast<uint8_t*>(p.Y) + m * p.ldy, n, p.N, h, most, s);
+    const Scale s(most);
+    if (p.group && n % p.group == 0 && n < p.N) p.scales[m * p.lds + (n >> p.group_shift)] = s.scale;
+    store_codes<VEC, AL>(static_cast<uint8_t*>(p.Y) + m * p.ldy, n, p.N, h,
+                         [&](int, float y) { return s(y); });
   }
 }
 
@@ -435,7 +488,7 @@ cudaError_t dispatch_aligned(const RmsNormArgs& p, cudaStream_t st) {
   auto same = [](const void* q, int64_t ld, int64_t ldx, int bytes) {
     return (reinterpret_cast<uintptr_t>(q) % bytes) == 0 && (ld - ldx) % VEC == 0;
   };
-  const bool cut = p.group == 0 && same(p.X, p.ldx, p.ldx, 16) &&
+  const bool cut = same(p.X, p.ldx, p.ldx, 16) &&
                    (!p.R || same(p.R, p.ldr, p.ldx, 16)) && (!p.H || same(p.H, p.ldh, p.ldx, 16)) &&
                    same(p.Y, p.ldy, p.ldx, p.scales ? VEC : 16);
   return cut ? dispatch<T, kCut>(p, st) : dispatch<T, kAnyhow>(p, st);

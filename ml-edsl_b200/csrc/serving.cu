@@ -96,6 +96,7 @@ int b200_rms_norm(const void* X, int64_t ldx, const void* R, int64_t ldr, int dt
   p.eps = eps;
   p.w_f32 = w && w_dtype == kF32;
   p.group = group;
+  p.group_shift = group == 32 ? 5 : group == 64 ? 6 : 7;
   return done(rms_norm(p, dtype, static_cast<cudaStream_t>(stream)), "rms_norm");
 }
 

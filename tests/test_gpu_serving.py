@@ -148,6 +148,16 @@ def test_rms_norm_extreme_rows(cuda):
     assert torch.isnan(y[5]).all() and torch.isnan(q[5].float()).all()
 
 
+@pytest.mark.parametrize("w", [1e37, 1e-33, 1e-36, 0.0])
+@pytest.mark.parametrize("N,group", [(512, 0), (512, 32), (301, 64), (301, 0)])
+def test_rms_norm_codes_of_extreme_weights(cuda, w, N, group):
+    x = rand(cuda, 1, 9, N)
+    weight = torch.full((N,), w, device=cuda)
+    q, s = serving.rms_norm(x, weight, quant="e4m3", group=group)
+    synced()
+    check_codes(q, s, norm_formula(x, weight, None, 1e-6), group)
+
+
 def test_rms_norm_shapes(cuda):
     x = rand(cuda, 1, 2, 3, 64).half()
     y = serving.rms_norm(x, None)
