@@ -14,11 +14,10 @@
 // bf16 parts of 8 bits each (exact), in three columns that are added at the
 // end. No product is rounded; sums run in f32, in the tensor core within a
 // group (or a 64-long part of one), then with ordinary adds after the scale
-// is applied in f32. An accumulator in TMEM would hold 128 columns of W by at
-// least 8 rows of X, but its operands have to come from shared memory, and
-// weights that are used once, by few rows, would be written there expanded
-// four times only to be read again; here they go from HBM to registers and
-// into the product.
+// is applied in f32. For up to 8 operand columns the codes go from HBM to
+// registers and into the product within one warp; more columns are
+// dense_w4_tc.cu's, where tcgen05 takes 16 to 128 of them at the price of
+// handing the expanded weights from one warp to another.
 //
 // Layout (w4_pack): strips of 64 columns; in a strip, blocks of 64 of K; in a
 // block, four 512-byte pieces of 16 columns, 16 bytes for each lane: the
@@ -159,18 +158,23 @@ __global__ void w4_dequantize_kernel(const uint32_t* __restrict__ codes, const c
 // ------------------------------------------------------------------ product
 
 // Few rows: a CTA has one strip of 64 columns and at most 8 operand columns,
-// and its four warps split the blocks of its part of K. Every lane
-// copies the codes that it will use itself, kDepth blocks ahead, into shared
-// memory (cp.async), so the loop over K has no barrier; scales and zeros are
-// one block ahead in registers. The activations of the CTA's part of K are
-// staged once, or stage_blocks of K at a time where that takes more than
-// kXBytes. CTAs are small so that several share an SM and the last wave is
-// short; the CTAs of a cluster share K.
-constexpr int kFewWarps = 4;
+// and its eight warps split the blocks of its part of K; the CTAs of a cluster
+// share K. Every lane copies the codes that it will use itself, kDepth blocks
+// ahead, into shared memory (cp.async), so the loop over K has no barrier;
+// scales follow one block behind in registers. The activations of the CTA's
+// part of K are staged once, or stage_blocks of K at a time where that takes
+// more than kXBytes.
+//
+// Bound by issue, not yet by HBM: about 340 instructions for a block and strip
+// (4096 weights: 176 to expand them, 16 products, 16 sums, the rest copies and
+// addresses) keep the schedulers at 45%. 1x4096x4096 bf16 5.3 us (floor 1.3),
+// 1x8192x16384 22.5 us or 3.1 TB/s (floor 10.6); with four warps a CTA and four
+// CTAs an SM 5.7 and 26.5 us, with six blocks ahead 32.5 us for the latter.
+constexpr int kFewWarps = 8;
 constexpr int kFewColumns = 8;  // operand columns of a CTA
 constexpr int kDepth = 4;
 constexpr int kXBytes = 24 * 1024;
-constexpr int kFewCtas = 4;  // an SM: with five, 96 registers spill (1x4096x4096 5.8 -> 6.5 us)
+constexpr int kFewCtas = 2;  // an SM
 
 template <int XT, bool FINE>
 __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas)

@@ -389,9 +389,15 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
     }
   }
 
+  __syncwarp();
+  // TMEM goes back before this CTA waits for others: two clusters that share
+  // SMs must not hold it while each waits for a CTA that waits for it
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (wid == kMmaWarp) tmem_dealloc(tmem, 512);
   // ---- the CTAs' parts of K: each 32 outputs of a row belong to one CTA of
   // the cluster, in turn
-  __syncwarp();
   const int chunks = mrows * 4;
   const int slots = ((chunks + C - 1) >> log_c) * 32;
   if (C > 1) cluster.barrier_wait();  // every CTA of the cluster runs
@@ -410,11 +416,8 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
       }
     }
   }
-  tc_fence_before();
   if (C > 1) cluster.sync();
   else __syncthreads();
-  tc_fence_after();
-  if (wid == kMmaWarp) tmem_dealloc(tmem, 512);
   // four outputs a thread
   const int64_t y_bytes = a.y_dtype == kF32 ? 4 : 2;
   const bool whole = reinterpret_cast<uintptr_t>(a.Y) % (4 * y_bytes) == 0 && a.ldy % 4 == 0;
