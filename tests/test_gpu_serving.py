@@ -326,7 +326,8 @@ def check_tokens(out, logits, tokens, top):
     p = torch.softmax(x, 1)
     entropy = -torch.special.xlogy(p, p).sum(1)
     # e^t to 2 + 1.2 |t| steps of 2^-23, |t| e^t <= 0.37; sums of at most
-    # V / 512 + 4 terms in a thread and 16 joins; each join rescales (4 steps)
+    # V / 256 terms in a thread, half a step each (V / 512 steps), and 16 joins;
+    # each join rescales (4 steps)
     s_err = (V / 512 + 4 + 16 * 5 + 8) * 2.0 ** -23
     span = (x.amax(1) - lse).abs() + 1
     if tokens is not None:
