@@ -57,8 +57,15 @@ __device__ __forceinline__ float row_reduce(float v, float* sh) {
 // odd length in a buffer that starts on 16 bytes, each with the same cut off
 // 16 bytes in every tensor. A cut row's chunks are those of the memory, so
 // that all but its first and last one are 16-byte accesses (4234x7710 f32 with
-// residual to e4m3: 163 us element by element, 87 us cut; floor 65).
+// residual to e4m3: 163 us element by element, 95 us cut; floor 65).
 enum Rows { kAligned, kAnyhow, kCut };
+
+// Chunks that lie outside the row altogether are told apart first: a thread may
+// have several of them, and going through one element by element costs more
+// than a whole one.
+__device__ __forceinline__ bool outside(int64_t n, int vec, int64_t N) {
+  return n >= N || n + vec <= 0;
+}
 
 // Elements [n, n + VEC) of a row as floats, 0 past N (and before 0).
 template <class T, bool AL>
@@ -67,6 +74,9 @@ __device__ __forceinline__ void load_chunk(const T* row, int64_t n, int64_t N, f
   if (AL && n >= 0 && n + VEC <= N) {
     // an ordinary load: h may be stored over x or over the residual
     unpack(*reinterpret_cast<const uint4*>(row + n), (const T*)nullptr, f);
+  } else if (outside(n, VEC, N)) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = 0.0f;
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) f[i] = n + i >= 0 && n + i < N ? to_f32(row[n + i]) : 0.0f;
@@ -80,7 +90,7 @@ __device__ __forceinline__ void store_chunk(T* row, int64_t n, int64_t N, const 
     // streaming: outputs do not push the rows that are still to be read out of
     // L2 (65536x4096 bf16 with residual: 370 -> 357 us; loads gain nothing)
     __stcs(reinterpret_cast<uint4*>(row + n), pack(f, (const T*)nullptr));
-  } else {
+  } else if (!outside(n, VEC, N)) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
       if (n + i >= 0 && n + i < N) row[n + i] = from_f32<T>(f[i]);
@@ -107,6 +117,7 @@ __device__ __forceinline__ void load_weight(const RmsNormArgs& p, int64_t n, flo
 template <int VEC, bool AL, class Factor>
 __device__ __forceinline__ void store_codes(uint8_t* row, int64_t n, int64_t N, const float* y,
                                             Factor factor) {
+  if (outside(n, VEC, N)) return;
   float c[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) c[i] = factor(i, y[i]);
@@ -179,6 +190,8 @@ struct RawChunk {
     constexpr int VEC = Chunk<T>::kElems;
     if (n >= 0 && n + VEC <= N) {
       v = *reinterpret_cast<const uint4*>(row + n);
+    } else if (outside(n, VEC, N)) {
+      v = make_uint4(0, 0, 0, 0);
     } else {
       float f[VEC];
 #pragma unroll
@@ -192,6 +205,11 @@ template <class T>
 struct RawChunk<T, false> {
   float v[Chunk<T>::kElems];
   __device__ __forceinline__ void load(const T* row, int64_t n, int64_t N) {
+    if (n >= N) {
+#pragma unroll
+      for (int i = 0; i < Chunk<T>::kElems; ++i) v[i] = 0.0f;
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < Chunk<T>::kElems; ++i) v[i] = n + i < N ? to_f32(row[n + i]) : 0.0f;
   }
@@ -211,7 +229,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
   constexpr bool AL = HOW != kAnyhow, WHOLE = HOW == kAligned;
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1;
   __shared__ float sh[2][3][32];  // in turn, for one row and the next
-  constexpr int kRowGroups = ROWS > 1 ? 33 : 1025;  // of 32 columns
+  constexpr int kRowGroups = ROWS > 1 ? 33 : 513;  // of 32 columns
   __shared__ uint32_t sh_groups[2][HOW == kCut ? ROWS * kRowGroups : 1];
   const int t = threadIdx.x % TPR;
   const int64_t step = (int64_t)gridDim.x * ROWS;
@@ -311,6 +329,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
       uint32_t* gm = sh_groups[odd] + threadIdx.x / TPR * kRowGroups;
       uint32_t* next = sh_groups[odd ^ 1] + threadIdx.x / TPR * kRowGroups;
       const int groups = (int)((p.N + p.group - 1) >> p.group_shift);
+      if (TPR == 32) __syncwarp();  // wider rows met at their sum
       for (int g = t; g < groups; g += TPR) next[g] = 0;  // the row before has been read
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -354,10 +373,11 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 
 // Rows that do not fit the registers of one CTA: the row is read once for the
 // sum, once more for a row's maximum, and once to be written.
-template <class T, bool AL>
+template <class T, Rows HOW>
 __global__ void __launch_bounds__(1024)
     rms_norm_long_kernel(const __grid_constant__ RmsNormArgs p) {
   constexpr int VEC = Chunk<T>::kElems, TPR = 1024;
+  constexpr bool AL = HOW != kAnyhow, WHOLE = HOW == kAligned;
   __shared__ float sh[3][32];
   const int t = threadIdx.x;
   const int64_t m = blockIdx.x;
@@ -365,12 +385,13 @@ __global__ void __launch_bounds__(1024)
   pdl_wait();
   const T* x = static_cast<const T*>(p.X) + m * p.ldx;
   const T* r = p.R ? static_cast<const T*>(p.R) + m * p.ldr : nullptr;
-  const int64_t chunks = (p.N + VEC - 1) / VEC;
+  const int cut = HOW == kCut ? (int)(m * p.ldx & (VEC - 1)) : 0;
+  const int64_t chunks = (p.N + cut + VEC - 1) / VEC;
   auto load_h = [&](int64_t c, float* h) {
-    load_chunk<T, AL>(x, c * VEC, p.N, h);
+    load_chunk<T, AL>(x, c * VEC - cut, p.N, h);
     if (r) {
       float f[VEC];
-      load_chunk<T, AL>(r, c * VEC, p.N, f);
+      load_chunk<T, AL>(r, c * VEC - cut, p.N, f);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) h[i] += f[i];
     }
@@ -395,7 +416,7 @@ __global__ void __launch_bounds__(1024)
     for (int64_t j = t; j < chunks; j += TPR) {
       float h[VEC], w[VEC];
       load_h(j, h);
-      load_weight<T, AL>(p, j * VEC, w);
+      load_weight<T, WHOLE>(p, j * VEC - cut, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) all = fmaxf(all, fabsf(h[i] * f.pre * f.inv * w[i]));
     }
@@ -404,10 +425,10 @@ __global__ void __launch_bounds__(1024)
   }
   // whole warps take part in every step: a group's lanes exchange their maxima
   for (int64_t j0 = 0; j0 < chunks; j0 += TPR) {
-    const int64_t n = (j0 + t) * VEC;
+    const int64_t n = (j0 + t) * VEC - cut;
     float h[VEC], w[VEC];
     load_h(j0 + t, h);
-    load_weight<T, AL>(p, n, w);
+    load_weight<T, WHOLE>(p, n, w);
     if (p.H) store_chunk<T, AL>(static_cast<T*>(p.H) + m * p.ldh, n, p.N, h);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) h[i] = h[i] * f.pre * f.inv * w[i];
@@ -465,14 +486,32 @@ template <class T, Rows HOW>
 cudaError_t dispatch(const RmsNormArgs& p, cudaStream_t st) {
   constexpr int VEC = Chunk<T>::kElems;
   const int64_t c = (p.N + (HOW == kCut ? VEC - 1 : 0) + VEC - 1) / VEC;
+  // Few rows: time is latency, so a thread has one chunk (148x800 bf16, plain and
+  // with residual to e4m3: 1.9 and 2.2 us, with four chunks 3.0 and 4.4;
+  // 148x4096: 2.1 and 2.6, with two chunks 2.4 and 3.0). More rows than CTAs
+  // stay at once: what counts is how many rows are under way, so a row has the
+  // fewest threads that hold it with two chunks each, or four of a warp
+  // (8192x800: 8.8 and 16.0 us, with 128 threads 13.1 and 22.3; 1024x800, which
+  // all run at once: 3.6 and 5.1 us, with 128 threads 2.8 and 4.0). The steps
+  // between the powers of two: 8192x2056 25.4 -> 20.5 us, 8192x4104 48.8 -> 41.1,
+  // 8192x8200 96.8 -> 84.5. Four chunks of 1024 threads are no faster than
+  // reading the row twice (4096x32768 bf16 216 and 179 us).
+  const bool few = p.M <= 148, wave = p.M <= 148 * 8;
   if (c <= 32) return launch<T, 32, 1, HOW>(p, st);
-  if (c <= 128) return launch<T, 32, 4, HOW>(p, st);
+  if (c <= 256 && few) return launch<T, 256, 1, HOW>(p, st);
+  if (c <= 512 && few) return launch<T, 512, 1, HOW>(p, st);
+  if (c <= 128 && !wave) return launch<T, 32, 4, HOW>(p, st);
   if (c <= 256) return launch<T, 128, 2, HOW>(p, st);
+  if (c <= 384) return launch<T, 192, 2, HOW>(p, st);
   if (c <= 512) return launch<T, 256, 2, HOW>(p, st);
+  if (c <= 768) return launch<T, 384, 2, HOW>(p, st);
   if (c <= 1024) return launch<T, 512, 2, HOW>(p, st);
-  if (c <= 2048) return launch<T, 512, 4, HOW>(p, st);
-  if (c <= 4096) return launch<T, 1024, 4, HOW>(p, st);
-  return launch_kernel(rms_norm_long_kernel<T, HOW == kAligned>, (unsigned)p.M, 1024, p, st);
+  if (c <= 1536) return launch<T, 768, 2, HOW>(p, st);
+  if (c <= 2048) return launch<T, 1024, 2, HOW>(p, st);
+  // groups of cut rows: element by element
+  if (HOW == kCut && p.group)
+    return launch_kernel(rms_norm_long_kernel<T, kAnyhow>, (unsigned)p.M, 1024, p, st);
+  return launch_kernel(rms_norm_long_kernel<T, HOW>, (unsigned)p.M, 1024, p, st);
 }
 
 template <class T>

@@ -96,6 +96,32 @@ def test_rms_norm(cuda, dtype, M, N, residual, quant, group):
         assert ((out[0].double() - y).abs() <= half_step(y, dtype) + NORM_F32 * y.abs()).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M", [2, 149, 1190])
+@pytest.mark.parametrize("chunks", [32, 33, 130, 257, 385, 513, 769, 1025, 1537, 2049, 2500])
+@pytest.mark.parametrize("odd", [0, 1])
+def test_rms_norm_widths(cuda, dtype, M, chunks, odd):
+    """Rows of every number of 16-byte chunks where the threads of a row change,
+    few of them, as many as run at once and more; on 16 bytes and cut off it."""
+    if M * chunks > 1190 * 800:
+        M = 301  # more than the CTAs that a GPU runs of the widest rows
+    N = chunks * (4 if dtype == F32 else 8) - odd
+    x = (rand(cuda, N, M, N) * 2).to(dtype)
+    r = (rand(cuda, N + 1, M, N) * 3).to(dtype)
+    w = (rand(cuda, N + 2, N) * 0.3 + 1).to(dtype)
+    y, h = serving.rms_norm(x, w, residual=r, eps=1e-5)
+    rows, row_scales, h1 = serving.rms_norm(x, w, residual=r, eps=1e-5, quant="e4m3")
+    codes, scales, h2 = serving.rms_norm(x, w, residual=r, eps=1e-5, quant="e4m3", group=32)
+    synced()
+    for got in (h, h1, h2):
+        assert torch.equal(got, (x.float() + r.float()).to(dtype))
+    want = norm_formula(x, w, r, 1e-5)
+    assert ((y.double() - want).abs() <= half_step(want, dtype) + NORM_F32 * want.abs()).all()
+    check_codes(rows, row_scales, want, 0)
+    some = slice(0, M, max(1, M // 7))
+    check_codes(codes[some], scales[some], want[some], 32)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("N,more,offset", [(512, 8, 0), (512, 3, 0), (512, 8, 1), (1000, 0, 5)])
 def test_rms_norm_pitches_and_alignments(cuda, dtype, N, more, offset):
