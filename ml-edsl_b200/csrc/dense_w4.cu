@@ -40,9 +40,44 @@ cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
   if (allowed.load(std::memory_order_relaxed) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
   if (e == cudaSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
   return e;
+}
+
+Capacity::Capacity(const void* kernel, int threads, int smem) {
+  for (int l = 0; l < 4; ++l) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(8u * 148);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 1u << l;
+    at[0].val.clusterDim.y = 1;
+    at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int clusters = 0;
+    const bool known = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess;
+    ctas[l] = known && clusters > 0 ? (int64_t)clusters << l : l == 0 ? 148 : 0;
+  }
+}
+
+int choose_cluster(const Capacity& capacity, int64_t tiles, int64_t kblocks, int warps, int fixed) {
+  int best = 0;
+  int64_t least = INT64_MAX;
+  for (int l = 0; l <= 3; ++l) {
+    if (capacity.ctas[l] == 0) continue;
+    const int64_t waves = ((tiles << l) + capacity.ctas[l] - 1) / capacity.ctas[l];
+    const int64_t blocks = (kblocks + ((int64_t)warps << l) - 1) / ((int64_t)warps << l);
+    const int64_t cost = waves * (blocks + fixed);
+    if (cost < least) {
+      least = cost;
+      best = l;
+    }
+  }
+  return best;
 }
 
 namespace {
@@ -175,6 +210,7 @@ constexpr int kFewColumns = 8;  // operand columns of a CTA
 constexpr int kDepth = 4;
 constexpr int kXBytes = 24 * 1024;
 constexpr int kFewCtas = 2;  // an SM
+constexpr int kFewShared = 96 * 1024;  // at most: 64 copied ahead, kXBytes, sums
 
 template <int XT, bool FINE>
 __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas)
@@ -475,20 +511,11 @@ int launch_few(W4Params p, cudaStream_t st) {
   const int64_t tiles = p.a.w.strips();
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
   if (chunks > 65535) return kErrTooLarge;
-  // CTAs that share K: the fewest waves of the GPU's 148 * kFewCtas CTAs, each as
-  // long as a warp's blocks and kFixed of setting up and adding.
-  constexpr int kFixed = 4;
-  int best = 0;
-  int64_t least = INT64_MAX;
-  for (int l = 0; l <= 3; ++l) {
-    const int64_t waves = ((tiles * chunks << l) + 148 * kFewCtas - 1) / (148 * kFewCtas);
-    const int64_t blocks = (p.kblocks + (kFewWarps << l) - 1) / (kFewWarps << l);
-    const int64_t cost = waves * (blocks + kFixed);
-    if (cost < least) {
-      least = cost;
-      best = l;
-    }
-  }
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
+  if (e0 != cudaSuccess) return launch_result(e0);
+  static const Capacity capacity(reinterpret_cast<const void*>(kernel), kFewWarps * 32, kFewShared);
+  const int best = choose_cluster(capacity, tiles * chunks, p.kblocks, kFewWarps, 4);
   const int C = 1 << best;
   p.log_cluster = best;
   const int64_t mine = (p.kblocks + C - 1) / C;
@@ -499,9 +526,6 @@ int launch_few(W4Params p, cudaStream_t st) {
   p.recv_bytes = C * XRow<XT>::kParts * ((rows * 2 + C - 1) / C * 32) * 4;
   const int smem = p.recv_bytes + kFewWarps * kDepth * 2048 + cols * (p.stage_blocks * 128 + 64) +
                    128;  // and the zeros of columns that no row has
-  static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
-  if (e0 != cudaSuccess) return launch_result(e0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)chunks);
   cfg.blockDim = dim3(kFewWarps * 32);

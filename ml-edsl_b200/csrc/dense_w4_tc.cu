@@ -490,29 +490,17 @@ int launch(W4Params p, int* status, cudaStream_t st) {
   const int64_t tiles = (p.a.w.N + kTileN - 1) / kTileN;
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
   if (chunks > 65535) return kErrTooLarge;
-  // CTAs that share K: the fewest waves, each as long as a CTA's blocks and
-  // kFixed of setting up and adding.
-  constexpr int kFixed = 8;
-  int best = 0;
-  int64_t least = INT64_MAX;
-  for (int l = 0; l <= 3; ++l) {
-    const int64_t waves = ((tiles * chunks << l) + 148 - 1) / 148;
-    const int64_t blocks = (p.kblocks + (1 << l) - 1) >> l;
-    const int64_t cost = waves * (blocks + kFixed);
-    if (cost < least) {
-      least = cost;
-      best = l;
-    }
-  }
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
+  if (e0 != cudaSuccess) return launch_result(e0);
+  static const Capacity capacity(reinterpret_cast<const void*>(kernel), S::kThreads, kMaxShared);
+  const int best = choose_cluster(capacity, tiles * chunks, p.kblocks, 1, 8);
   const int C = 1 << best;
   p.log_cluster = best;
   const int rows = (int)std::min<int64_t>(p.rows, p.a.M);
   p.recv_bytes = C * PARTS * ((rows * 4 + C - 1) / C * 32) * 4;
   const int smem = S::kCount * S::kBlocks * NC * 128 + kExpanders * kCodeDepth * 1024 + p.recv_bytes +
                    (int)sizeof(Barriers);
-  static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
-  if (e0 != cudaSuccess) return launch_result(e0);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * C), (unsigned)chunks);
   cfg.blockDim = dim3(S::kThreads);

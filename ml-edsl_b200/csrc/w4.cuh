@@ -233,9 +233,25 @@ __device__ __forceinline__ void prefetch_l2_bulk(const void* p, uint32_t bytes) 
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes) : "memory");
 }
 
-// Lets `kernel` use 200 KB of dynamic shared memory on the current device.
+constexpr int kMaxShared = 200 * 1024;
+
+// Lets `kernel` use kMaxShared of dynamic shared memory on the current device.
 // `allowed`: one bit a device that has been told.
 cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed);
+
+// How many CTAs of `kernel` run at once in clusters of 1, 2, 4 and 8. GPUs
+// differ in how many clusters fit, so the driver is asked, once a kernel.
+struct Capacity {
+  int64_t ctas[4];
+  Capacity(const void* kernel, int threads, int smem);
+};
+
+// The log2 of the CTAs that share K, of `tiles` CTAs' work each `kblocks` long
+// that `warps` warps split: the fewest waves, each as long as a warp's blocks
+// and `fixed` of setting up and adding. Clusters of 8 take more waves than
+// their number of CTAs lets expect (16x16384x2048 bf16: 22.3 us, in clusters of
+// 4 18.4, alone 61; 16x4096x512: 5.3 us, in fours 7.0).
+int choose_cluster(const Capacity& capacity, int64_t tiles, int64_t kblocks, int warps, int fixed);
 
 // Many rows, on the tensor core (dense_w4_tc.cu).
 int dense_w4_tc(const W4Params& p, int* status, cudaStream_t st);
