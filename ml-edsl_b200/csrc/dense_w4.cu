@@ -277,15 +277,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, kFewCtas)
       zraw[sub] = __ldg(reinterpret_cast<const uint2*>(p.zeros + col0 + (int64_t)p.group_of(k) * 64));
     }
   };
-  // What the CTA will read of the weights is contiguous. The previous kernel of
-  // the stream may still run (and may have written them): until pdl_wait they
-  // are only brought into L2.
-  if (tid == 0 && b0 < b1)
-    prefetch_l2_bulk(p.codes + (strip * kblocks + b0) * 128, (uint32_t)min(b1 - b0, 64) * 2048u);
-  if (tid == 32 && b0 < b1) {
-    const int64_t at = strip * p.groups * 64 + (int64_t)p.group_of(b0 * kBlockK) * 64;
-    prefetch_l2(p.scales + (s32 ? at * 4 : at * 2));
-  }
+  // until pdl_wait the previous kernel of the stream may still run
+  if (tid == 0) prefetch_strip(p, strip, b0, b1, true);
   pdl_wait();
 
   // The activations that are staged first are asked for before the weights.

@@ -108,6 +108,9 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
     bar->abort_flag = 0;
     fence_barrier_init();
   }
+  // one thread for each of the CTA's strips
+  if (tid >= 32 && tid < 34 && n0 + (tid - 32) * kStripN < a.w.N)
+    prefetch_strip(p, n0 / kStripN + tid - 32, b0, b1, false);
   pdl_wait();
   if (wid == kMmaWarp) tmem_alloc(&bar->tmem, 512);
   tc_fence_before();

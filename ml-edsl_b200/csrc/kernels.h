@@ -1,5 +1,6 @@
 // Internal interface between the CUDA kernel files and the host runtime.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda_runtime.h>
 
@@ -24,6 +25,12 @@ enum RedOp : int { kRedSum = 0, kRedProd = 1, kRedMax = 2, kRedMin = 3 };
 
 // Number of kernels this library has launched (process-wide).
 void count_launch();
+
+constexpr int kMaxShared = 200 * 1024;
+
+// Lets `kernel` use kMaxShared of dynamic shared memory on the current device.
+// `allowed`: one bit a device that has been told.
+cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed);
 
 // Records an error for b200_last_error()/b200_last_status() on this thread
 // and returns `code`; report_ok() records success and returns kOk.

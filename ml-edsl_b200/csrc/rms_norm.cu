@@ -12,6 +12,7 @@
 // of at most 32 terms.
 #include <cuda_runtime.h>
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include "dtype.cuh"
 #include "kernels.h"
@@ -371,12 +372,18 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
   }
 }
 
-// Rows that do not fit the registers of one CTA: the row is read once for the
-// sum, once more for a row's maximum, and once to be written.
-template <class T, Rows HOW>
-__global__ void __launch_bounds__(1024)
+// Rows that do not fit the registers of one CTA. KEPT: h stays in shared memory,
+// in f32, each thread's chunks its own (4096x16383 f32 144 -> 128 us, floor 82;
+// 4096x32768 bf16 with residual to e4m3 396 -> 302 us, floor 143). Wider rows,
+// one CTA of which would fill an SM (2048x50000 f32 kept 256 us, otherwise 178),
+// are read once for the sum, once more for a row's maximum, and once to be
+// written.
+constexpr int kKeptBytes = 144 * 1024;
+template <class T, Rows HOW, bool KEPT>
+__global__ void __launch_bounds__(KEPT ? 512 : 1024)
     rms_norm_long_kernel(const __grid_constant__ RmsNormArgs p) {
-  constexpr int VEC = Chunk<T>::kElems, TPR = 1024;
+  constexpr int VEC = Chunk<T>::kElems, TPR = KEPT ? 512 : 1024;
+  extern __shared__ float4 kept[];  // [VEC / 4][chunk]
   constexpr bool AL = HOW != kAnyhow, WHOLE = HOW == kAligned;
   __shared__ float sh[3][32];
   const int t = threadIdx.x;
@@ -388,6 +395,17 @@ __global__ void __launch_bounds__(1024)
   const int cut = HOW == kCut ? (int)(m * p.ldx & (VEC - 1)) : 0;
   const int64_t chunks = (p.N + cut + VEC - 1) / VEC;
   auto load_h = [&](int64_t c, float* h) {
+    if (KEPT) {
+#pragma unroll
+      for (int i = 0; i < VEC / 4; ++i) {
+        const float4 v = c < chunks ? kept[i * chunks + c] : make_float4(0, 0, 0, 0);
+        h[4 * i] = v.x;
+        h[4 * i + 1] = v.y;
+        h[4 * i + 2] = v.z;
+        h[4 * i + 3] = v.w;
+      }
+      return;
+    }
     load_chunk<T, AL>(x, c * VEC - cut, p.N, h);
     if (r) {
       float f[VEC];
@@ -408,7 +426,42 @@ __global__ void __launch_bounds__(1024)
     }
     return row_reduce<Sum, TPR>(s, buf);
   };
-  const float ss = squares(1.0f, sh[0]);
+  float ss = 0.0f;
+  if (KEPT) {
+    constexpr int U = 4;  // chunks that a thread has under way
+    for (int64_t j0 = t; j0 < chunks; j0 += U * TPR) {
+      RawChunk<T, AL> xs[U], rs[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) xs[u].load(x, (j0 + u * TPR) * VEC - cut, p.N);
+      if (r) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) rs[u].load(r, (j0 + u * TPR) * VEC - cut, p.N);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t c = j0 + u * TPR;
+        if (c >= chunks) break;
+        float h[VEC];
+        xs[u].floats(h);
+        if (r) {
+          float f[VEC];
+          rs[u].floats(f);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) h[i] += f[i];
+        }
+        float part = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) part = fmaf(h[i], h[i], part);
+        ss += part;
+#pragma unroll
+        for (int i = 0; i < VEC / 4; ++i)
+          kept[i * chunks + c] = make_float4(h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]);
+      }
+    }
+    ss = row_reduce<Sum, TPR>(ss, sh[0]);
+  } else {
+    ss = squares(1.0f, sh[0]);
+  }
   const Factor f =
       factor(ss, (float)p.N, p.eps, [&](float c) { return squares(c, sh[1]); });
   float all = 0.0f;
@@ -453,11 +506,12 @@ __global__ void __launch_bounds__(1024)
 // Launches `kernel`, which may start early (it waits for the kernel before it
 // where it first reads memory).
 template <class Kernel>
-cudaError_t launch_kernel(Kernel kernel, unsigned grid, int threads, const RmsNormArgs& p,
-                          cudaStream_t st) {
+cudaError_t launch_kernel(Kernel kernel, unsigned grid, int threads, int smem,
+                          const RmsNormArgs& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -479,7 +533,22 @@ cudaError_t launch(const RmsNormArgs& p, cudaStream_t st) {
                : 1;
   }();
   const int64_t grid = std::min<int64_t>((p.M + ROWS - 1) / ROWS, (int64_t)148 * per_sm);
-  return launch_kernel(kernel, (unsigned)grid, THREADS, p, st);
+  return launch_kernel(kernel, (unsigned)grid, THREADS, 0, p, st);
+}
+
+template <class T, Rows HOW>
+cudaError_t launch_long(const RmsNormArgs& p, bool anyhow, cudaStream_t st) {
+  if constexpr (HOW == kCut) {
+    if (anyhow) return launch_long<T, kAnyhow>(p, false, st);
+  }
+  constexpr int VEC = Chunk<T>::kElems;
+  const int64_t bytes = ((p.N + VEC - 1 + (HOW == kCut ? VEC - 1 : 0)) / VEC) * VEC * 4;
+  if (bytes > kKeptBytes)
+    return launch_kernel(rms_norm_long_kernel<T, HOW, false>, (unsigned)p.M, 1024, 0, p, st);
+  auto kernel = rms_norm_long_kernel<T, HOW, true>;
+  static std::atomic<uint64_t> allowed{0};
+  const cudaError_t e = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
+  return e != cudaSuccess ? e : launch_kernel(kernel, (unsigned)p.M, 512, (int)bytes, p, st);
 }
 
 template <class T, Rows HOW>
@@ -494,8 +563,8 @@ cudaError_t dispatch(const RmsNormArgs& p, cudaStream_t st) {
   // (8192x800: 8.8 and 16.0 us, with 128 threads 13.1 and 22.3; 1024x800, which
   // all run at once: 3.6 and 5.1 us, with 128 threads 2.8 and 4.0). The steps
   // between the powers of two: 8192x2056 25.4 -> 20.5 us, 8192x4104 48.8 -> 41.1,
-  // 8192x8200 96.8 -> 84.5. Four chunks of 1024 threads are no faster than
-  // reading the row twice (4096x32768 bf16 216 and 179 us).
+  // 8192x8200 96.8 -> 84.5. Four chunks of 1024 threads are slower than
+  // rows in shared memory (4096x32768 bf16 216 and 179 us).
   const bool few = p.M <= 148, wave = p.M <= 148 * 8;
   if (c <= 32) return launch<T, 32, 1, HOW>(p, st);
   if (c <= 256 && few) return launch<T, 256, 1, HOW>(p, st);
@@ -509,9 +578,7 @@ cudaError_t dispatch(const RmsNormArgs& p, cudaStream_t st) {
   if (c <= 1536) return launch<T, 768, 2, HOW>(p, st);
   if (c <= 2048) return launch<T, 1024, 2, HOW>(p, st);
   // groups of cut rows: element by element
-  if (HOW == kCut && p.group)
-    return launch_kernel(rms_norm_long_kernel<T, kAnyhow>, (unsigned)p.M, 1024, p, st);
-  return launch_kernel(rms_norm_long_kernel<T, HOW>, (unsigned)p.M, 1024, p, st);
+  return launch_long<T, HOW>(p, HOW == kCut && p.group, st);
 }
 
 template <class T>
