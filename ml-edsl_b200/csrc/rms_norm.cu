@@ -58,7 +58,7 @@ __device__ __forceinline__ float row_reduce(float v, float* sh) {
 // odd length in a buffer that starts on 16 bytes, each with the same cut off
 // 16 bytes in every tensor. A cut row's chunks are those of the memory, so
 // that all but its first and last one are 16-byte accesses (4234x7710 f32 with
-// residual to e4m3: 163 us element by element, 95 us cut; floor 65).
+// residual to e4m3: 163 us element by element, 91 us cut; floor 65).
 enum Rows { kAligned, kAnyhow, kCut };
 
 // Chunks that lie outside the row altogether are told apart first: a thread may
@@ -112,6 +112,32 @@ __device__ __forceinline__ void load_weight(const RmsNormArgs& p, int64_t n, flo
     for (int i = 0; i < VEC; i += 4)
       load_chunk<float, AL>(static_cast<const float*>(p.w), n + i, p.N, f + i);
   }
+}
+
+// The weights of a chunk of a row that is cut off 16 bytes, n + cut a multiple of
+// VEC: out of the two aligned chunks of w that hold them (16384x5003 bf16 138 ->
+// 131 us, 4213x11811 bf16 with residual 125 -> 119; without weights 109 and 105).
+template <class T>
+__device__ __forceinline__ void load_weight_cut(const RmsNormArgs& p, int64_t n, int cut, float* f) {
+  constexpr int VEC = Chunk<T>::kElems;
+  const int64_t end = n + cut + VEC;  // of the second one
+  if (!p.w || (sizeof(T) == 2 && p.w_f32) || reinterpret_cast<uintptr_t>(p.w) % 16 != 0 || n < 0 ||
+      end > p.N)
+    return load_weight<T, false>(p, n, f);
+  if (cut == 0) return load_weight<T, true>(p, n, f);
+  const uint4* at = reinterpret_cast<const uint4*>(static_cast<const T*>(p.w) + (end - 2 * VEC));
+  const uint4 a = at[0], b = at[1];
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  // 16 bytes from `from` on, by two words, one and a half
+  const int from = 16 - cut * (int)sizeof(T);
+  uint32_t u[6], v[5], o[4];
+#pragma unroll
+  for (int i = 0; i < 6; ++i) u[i] = from & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = from & 4 ? u[i + 1] : u[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = __funnelshift_r(v[i], v[i + 1], (from & 2) * 8);
+  unpack(make_uint4(o[0], o[1], o[2], o[3]), (const T*)nullptr, f);
 }
 
 // Codes of VEC values; factor(i) scales value i into e4m3's range.
@@ -220,11 +246,17 @@ struct RawChunk<T, false> {
   }
 };
 
+// CTAs that the compiler has to leave registers for: cut rows take more of them
+// than pays (1000x1001 f32 3.4 -> 3.1 us).
+constexpr int ctas_at_once(int tpr, Rows how) {
+  return how != kCut ? 0 : tpr == 32 ? 4 : 1024 / tpr;  // 0: the compiler's choice
+}
+
 // Rows by TPR threads each, E chunks of 16 bytes a thread: chunk e * TPR + t of
 // a row is thread t's e-th. A row is read once and stays in registers; the next
 // row of the CTA is on its way while one is summed, scaled and stored.
 template <class T, int TPR, int E, Rows HOW>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, ctas_at_once(TPR, HOW))
     rms_norm_kernel(const __grid_constant__ RmsNormArgs p) {
   constexpr int VEC = Chunk<T>::kElems;
   constexpr bool AL = HOW != kAnyhow, WHOLE = HOW == kAligned;
@@ -293,7 +325,8 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       float w[VEC];
-      load_weight<T, WHOLE>(p, (int64_t)(e * TPR + t) * VEC - cut, w);
+      if (HOW == kCut) load_weight_cut<T>(p, (int64_t)(e * TPR + t) * VEC - cut, cut, w);
+      else load_weight<T, WHOLE>(p, (int64_t)(e * TPR + t) * VEC, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) h[e][i] = h[e][i] * f.pre * f.inv * w[i];
     }
@@ -373,7 +406,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR)
 }
 
 // Rows that do not fit the registers of one CTA. KEPT: h stays in shared memory,
-// in f32, each thread's chunks its own (4096x16383 f32 144 -> 128 us, floor 82;
+// in f32, each thread's chunks its own (4096x16383 f32 144 -> 121 us, floor 82;
 // 4096x32768 bf16 with residual to e4m3 396 -> 302 us, floor 143). Wider rows,
 // one CTA of which would fill an SM (2048x50000 f32 kept 256 us, otherwise 178),
 // are read once for the sum, once more for a row's maximum, and once to be
@@ -469,7 +502,8 @@ __global__ void __launch_bounds__(KEPT ? 512 : 1024)
     for (int64_t j = t; j < chunks; j += TPR) {
       float h[VEC], w[VEC];
       load_h(j, h);
-      load_weight<T, WHOLE>(p, j * VEC - cut, w);
+      if (HOW == kCut) load_weight_cut<T>(p, j * VEC - cut, cut, w);
+      else load_weight<T, WHOLE>(p, j * VEC, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) all = fmaxf(all, fabsf(h[i] * f.pre * f.inv * w[i]));
     }
@@ -481,7 +515,8 @@ __global__ void __launch_bounds__(KEPT ? 512 : 1024)
     const int64_t n = (j0 + t) * VEC - cut;
     float h[VEC], w[VEC];
     load_h(j0 + t, h);
-    load_weight<T, WHOLE>(p, n, w);
+    if (HOW == kCut) load_weight_cut<T>(p, n, cut, w);
+    else load_weight<T, WHOLE>(p, n, w);
     if (p.H) store_chunk<T, AL>(static_cast<T*>(p.H) + m * p.ldh, n, p.N, h);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) h[i] = h[i] * f.pre * f.inv * w[i];
