@@ -60,6 +60,7 @@ Capacity::Capacity(const void* kernel, int threads, int smem) {
     cfg.numAttrs = 1;
     int clusters = 0;
     const bool known = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess;
+    if (!known) cudaGetLastError();  // the next launch is not to report it
     ctas[l] = known && clusters > 0 ? (int64_t)clusters << l : l == 0 ? 148 : 0;
   }
 }

@@ -151,6 +151,26 @@ def test_rms_norm_residual_in_place(cuda, N, into):
     assert torch.equal(a if into == "x" else b, want_h)
 
 
+@pytest.mark.parametrize("N", [20001, 36000])
+def test_rms_norm_long_rows_in_place_and_out_of_range(cuda, N):
+    """Rows in shared memory: h over x, squares out of f32's range, zeros, a NaN."""
+    x, r = rand(cuda, 1, 5, N), rand(cuda, 2, 5, N)
+    x[1] *= 1e30
+    x[2], r[2] = 0, 0
+    x[3, N - 1] = NAN
+    h = x + r
+    want = norm_formula(x, None, r, 1e-6)
+    y, got = serving.rms_norm(x, None, residual=r, residual_out=x)
+    synced()
+    assert got.data_ptr() == x.data_ptr()
+    for row in (0, 1, 2, 4):
+        assert torch.equal(x[row], h[row])
+        err = (y[row].double() - want[row]).abs()
+        # the sum: at most 18 partial sums of four in a thread, within the 32 above
+        assert (err <= NORM_F32 * want[row].abs() + 2.0 ** -149).all(), row
+    assert torch.isnan(y[3]).all()
+
+
 def test_rms_norm_extreme_rows(cuda):
     """Squares out of f32's range, zeros, subnormal values, infinities, NaN."""
     N = 512
