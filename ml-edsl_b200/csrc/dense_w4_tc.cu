@@ -232,13 +232,13 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
       const int k0 = b0 * kBlockK + c * 8;
       const int64_t step = (int64_t)rows_step * a.ldx * 2;
       const char* from = x + ((int64_t)row0 * a.ldx + k0) * 2;
-      int left = (K - k0) * 2;      // bytes of the row from here on
+      int left = K - k0;            // elements of the row from here on; K may reach 2^31 - 64
       int64_t at_start = x - from;  // a valid address where nothing is read
       for (int t = 0; t < stages; ++t) {
         if (!reusable(t)) break;
 #pragma unroll
         for (int sb = 0; sb < SB; ++sb) {
-          const int bytes = max(0, min(16, left));
+          const int bytes = max(0, min(8, left)) * 2;
           char* to = place(t * SB + sb, row0);  // rows_step is a multiple of the swizzle's 8
 #pragma unroll
           for (int u = 0; u < PER; ++u)
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
                               bytes);
           from += kBlockK * 2;
           at_start -= kBlockK * 2;
-          left -= kBlockK * 2;
+          left -= kBlockK;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         post(t);

@@ -1,0 +1,49 @@
+"""The serving operators at the edges of what they take: the longest rows, values
+at both ends of f32's range, buffers that overlap, waits that run out."""
+import math
+
+import pytest
+import torch
+
+from mlir_edsl import _native, serving
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16, E4M3 = torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn
+INF, NAN = math.inf, math.nan
+
+
+def rand(cuda, seed, *shape):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    return torch.randn(*shape, device=cuda, generator=g)
+
+
+def synced():
+    torch.cuda.synchronize()
+    _native.check(_native.lib().b200_stream_sync(None))
+
+
+def test_dense_w4_rows_past_2_to_30(cuda):
+    """A row's bytes pass 2^31: every element counts, the first and last blocks'
+    among them. Whole numbers, so the sums are exact."""
+    K = (1 << 30) + 320
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 72 << 30:
+        pytest.skip("needs 72 GB of device memory")
+    x = torch.zeros(9, K, dtype=BF16, device=cuda)
+    at = [0, 70, 319, 320, K // 2, K - 321, K - 1]
+    for i, k in enumerate(at):
+        x[:, k] = 1 << i
+    x[3, at[1]] = 0
+    codes = torch.full((K, 1), 9, dtype=torch.uint8, device=cuda)
+    w = serving.pack_w4(codes, torch.ones(2, 1, dtype=BF16, device=cuda), group=1 << 30)
+    del codes
+    try:
+        y = serving.dense_w4(x, w, out_dtype=F32)
+        synced()
+        want = torch.full((9, 1), 127.0, device=cuda)
+        want[3] -= 2
+        assert torch.equal(y, want)
+    finally:
+        del x, w
+        torch.cuda.empty_cache()
