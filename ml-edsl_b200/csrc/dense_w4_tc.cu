@@ -451,6 +451,7 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
     const float xs = a.x_scales && a.x_group == 0 ? __ldg(a.x_scales + (m0 + m) * a.ldxs) : 1.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      y[i] *= Mma::kUp;
       if (a.x_scales && a.x_group == 0) y[i] *= xs;
       if (a.b && n + i < a.w.N) y[i] += load_as_f32(a.b, a.b_dtype, n + i);
       y[i] = activate(y[i], a.act, a.alpha);

@@ -47,3 +47,24 @@ def test_dense_w4_rows_past_2_to_30(cuda):
     finally:
         del x, w
         torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M", [1, 2, 3, 9, 70])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_dense_w4_sums_past_the_range(cuda, dtype, M, group):
+    """Sums of x * (code - zero) that leave f32's range while those of x * W stay in
+    it. Terms of one sign: a sum of absolute products is the sum itself, so its
+    error is below 2^-18 of it (16 k16 steps of two truncations, 2^-22 each, no more
+    than 8 of them in one sum; 8 + 16 additions)."""
+    K, N = 256, 70
+    codes = torch.full((K, N), 15, dtype=torch.uint8, device=cuda)
+    zeros = torch.zeros(-(-K // group), N, dtype=torch.uint8, device=cuda)
+    scales = torch.full(zeros.shape, 2.0 ** -16, device=cuda)
+    w = serving.pack_w4(codes, scales, zeros, group=group)
+    for value in (3e38, -1e38, 1e30):
+        x = torch.full((M, K), value, device=cuda).to(dtype)
+        y = serving.dense_w4(x, w, out_dtype=F32)
+        synced()
+        want = x.double().sum(1, keepdim=True) * (15 * 2.0 ** -16)
+        assert ((y.double() - want).abs() <= 2.0 ** -18 * want.abs()).all()
