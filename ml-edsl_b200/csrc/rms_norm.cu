@@ -196,16 +196,18 @@ __device__ __forceinline__ float group_max(float v, int lanes) {
 }
 
 // y = (h * pre) * inv with inv = 1 / sqrt(mean of squares + eps) and pre = 1.
-// The squares of |h| > 1.8e19 leave f32's range: pre is then 2^-100 and inv
-// that of h * pre (`squares(pre)` sums them over the row again).
+// The squares of |h| > 1.8e19 leave f32's range: inv is then that of h * 2^-100
+// (`squares(c)` sums those of h * c over the row again), and its 2^-100 goes to
+// both factors so that neither leaves the range: an h that pre makes subnormal has
+// a y that is.
 struct Factor {
   float pre, inv;
 };
 template <class Fn>
 __device__ __forceinline__ Factor factor(float ss, float N, float eps, Fn squares) {
   if (ss < __int_as_float(0x7f800000)) return {1.0f, 1.0f / sqrtf(ss / N + eps)};
-  const float c = 7.88860905e-31f;
-  return {c, 1.0f / sqrtf(squares(c) / N + eps * c * c)};
+  const float c = 0x1p-100f;
+  return {0x1p-48f, 0x1p-52f / sqrtf(squares(c) / N + eps * c * c)};
 }
 
 // A chunk of x (and of r) as it lies in memory, or as floats where it has to be

@@ -68,3 +68,40 @@ def test_dense_w4_sums_past_the_range(cuda, dtype, M, group):
         synced()
         want = x.double().sum(1, keepdim=True) * (15 * 2.0 ** -16)
         assert ((y.double() - want).abs() <= 2.0 ** -18 * want.abs()).all()
+
+
+# as in the tests of ordinary rows: 49 roundings of the sum, halved by the root,
+# and six more; one of these is that of a row's second factor
+NORM_F32 = 2.0 ** -19
+
+
+def norm_formula(x, eps):
+    h = x.double()
+    return h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps)
+
+
+def half_step(v, dtype):
+    tiny = {F32: 2.0 ** -150, BF16: 2.0 ** -134}[dtype]
+    return (v.abs() * (torch.finfo(dtype).eps / 2)).clamp(min=tiny)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N", [301, 512, 4096, 20001, 50000])
+def test_rms_norm_of_small_values_beside_large_ones(cuda, dtype, N):
+    """A row whose squares leave f32's range keeps the bits of its small values."""
+    x = rand(cuda, N, 5, N) * 1e-12
+    x[0, 0], x[1, N - 1], x[2, 7], x[3, 9] = 2e19, -3e38, 1e25, 5e19
+    x[4, ::3] = 1e22
+    x = x.to(dtype)
+    y = serving.rms_norm(x)
+    q, s = serving.rms_norm(x, quant="e4m3", group=32)
+    synced()
+    want = norm_formula(x, 1e-6)
+    assert ((y.double() - want).abs() <= half_step(want, dtype) + NORM_F32 * want.abs()).all()
+    for i, g0 in enumerate(range(0, N, 32)):
+        most = want[:, g0:g0 + 32].abs().amax(1)
+        scale = s[:, i].double()
+        # a scale below half of f32's smallest value is 0 there, and 1 stands for 0
+        none = (most / 448 < 2.0 ** -149) & (scale == 1)
+        room = 2 * NORM_F32 * most / 448 + 2.0 ** -149
+        assert (none | ((scale - most / 448).abs() <= room)).all()
