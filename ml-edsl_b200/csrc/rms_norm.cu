@@ -196,18 +196,22 @@ __device__ __forceinline__ float group_max(float v, int lanes) {
 }
 
 // y = (h * pre) * inv with inv = 1 / sqrt(mean of squares + eps) and pre = 1.
-// The squares of |h| > 1.8e19 leave f32's range: inv is then that of h * 2^-100
-// (`squares(c)` sums those of h * c over the row again), and its 2^-100 goes to
-// both factors so that neither leaves the range: an h that pre makes subnormal has
-// a y that is.
+// `squares(c)` sums the squares of h * c over the row again, where those of h leave
+// f32's range: |h| > 1.8e19, with c = 2^-100, which then goes to both factors so
+// that neither leaves the range (an h that pre makes subnormal has a y that is);
+// or |h| < 2^-45 with an eps that does not hide what its squares lose, with
+// c = 2^60.
 struct Factor {
   float pre, inv;
 };
 template <class Fn>
 __device__ __forceinline__ Factor factor(float ss, float N, float eps, Fn squares) {
-  if (ss < __int_as_float(0x7f800000)) return {1.0f, 1.0f / sqrtf(ss / N + eps)};
-  const float c = 0x1p-100f;
-  return {0x1p-48f, 0x1p-52f / sqrtf(squares(c) / N + eps * c * c)};
+  const float tiny = 0x1p-90f;
+  const bool small = ss < tiny && eps < tiny;
+  if (ss < __int_as_float(0x7f800000) && !small) return {1.0f, 1.0f / sqrtf(ss / N + eps)};
+  const float c = small ? 0x1p60f : 0x1p-100f;
+  const float inv = 1.0f / sqrtf(squares(c) / N + eps * c * c);
+  return small ? Factor{c, inv} : Factor{0x1p-48f, 0x1p-52f * inv};
 }
 
 // A chunk of x (and of r) as it lies in memory, or as floats where it has to be

@@ -105,3 +105,17 @@ def test_rms_norm_of_small_values_beside_large_ones(cuda, dtype, N):
         none = (most / 448 < 2.0 ** -149) & (scale == 1)
         room = 2 * NORM_F32 * most / 448 + 2.0 ** -149
         assert (none | ((scale - most / 448).abs() <= room)).all()
+
+
+@pytest.mark.parametrize("N", [301, 512, 4096, 20001, 50000])
+def test_rms_norm_of_tiny_rows_and_eps(cuda, N):
+    """Squares below f32's range, with an eps that does not hide them."""
+    eps = float(torch.tensor(1e-42))
+    x = rand(cuda, N, 4, N) * 1e-21
+    x[1] *= 1e-3
+    x[2] = 0
+    x[3] *= 1e5
+    y = serving.rms_norm(x, eps=eps)
+    synced()
+    want = norm_formula(x, eps)
+    assert ((y.double() - want).abs() <= half_step(want, F32) + NORM_F32 * want.abs()).all()
