@@ -391,6 +391,14 @@ int b200_dense_w4(const void* X, int64_t ldx, int x_dtype, const float* x_scales
                   int group, const void* b, int b_dtype, void* Y, int64_t ldy, int y_dtype,
                   int64_t M, int64_t N, int64_t K, int act, float alpha, void* stream);
 
+/* The tensor core's kernel bounds the waits between its warps (2 s). If one runs
+ * out, the results of the CTAs that share its part of Y are NaN and the next
+ * b200_stream_sync on the device returns B200_ERR_DEVICE_TIMEOUT.
+ * b200_debug_w4_expire(limit_ns) makes that happen, for tests: from the next
+ * launch on (process-wide) products do not report their end, and waits run out
+ * after limit_ns; 0 restores both. */
+int b200_debug_w4_expire(int64_t limit_ns);
+
 /* 4-bit weights of a host matrix, kept on each GPU like b200_weights_register
  * keeps f32 ones: b200_weights_register_w4 declares the f32 W[K,N] at host
  * address W unchanged until it is registered with another version (or shape

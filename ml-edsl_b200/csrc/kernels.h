@@ -222,6 +222,7 @@ struct DenseW4Args {
   float alpha;
 };
 int dense_w4(const DenseW4Args& p, int* status, cudaStream_t st);
+void w4_expire(int64_t limit_ns);  // b200_debug_w4_expire
 int w4_quantize(const float* W, int64_t ldw, int64_t K, int64_t N, int group, uint8_t* codes,
                 int64_t ldc, void* scales, int64_t lds, int s_dtype, cudaStream_t st);
 int w4_pack(const uint8_t* codes, int64_t ldc, const void* scales, int64_t lds,

@@ -89,30 +89,57 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* s
   return mbar_wait_for(bar, parity, status, code, abort_flag, B200_WAIT_NS);
 }
 
-// mbar_wait for kernels with many waiting warps: each try may suspend the warp
-// for up to 20 us, so that waiting costs next to no issue slots.
+// For kernels with many waiting warps: a try that may suspend the warp for up to
+// 20 us, so that waiting costs next to no issue slots.
+__device__ __forceinline__ bool mbar_try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
+
+// mbar_wait of one thread with such tries.
 __device__ __forceinline__ bool mbar_wait_long(uint64_t* bar, uint32_t parity, int* status,
-                                               int code, volatile int* abort_flag) {
+                                               int code, volatile int* abort_flag,
+                                               uint64_t limit_ns) {
   if (mbar_try_wait(bar, parity)) return true;
   uint64_t start = 0;
   while (true) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
-        : "memory");
-    if (ok) return true;
+    if (mbar_try_wait_long(bar, parity)) return true;
     if (*abort_flag) return false;
     const uint64_t now = globaltimer();
     if (start == 0) start = now;
-    if (now - start > B200_WAIT_NS) {
+    if (now - start > limit_ns) {
       if (status) atomicCAS(status, 0, code);
       *abort_flag = 1;
       return false;
     }
+  }
+}
+
+// The same by a whole warp, with one answer for all lanes: what follows may be a
+// warp's collective operation.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* status,
+                                               int code, volatile int* abort_flag,
+                                               uint64_t limit_ns) {
+  constexpr uint32_t kAll = 0xffffffffu;
+  if (__all_sync(kAll, mbar_try_wait(bar, parity))) return true;
+  uint64_t start = 0;
+  while (true) {
+    if (__all_sync(kAll, mbar_try_wait_long(bar, parity))) return true;
+    const uint64_t now = globaltimer();
+    if (start == 0) start = now;
+    const bool over = now - start > limit_ns;
+    if (over) {
+      if (status) atomicCAS(status, 0, code);
+      *abort_flag = 1;
+    }
+    if (__any_sync(kAll, over || *abort_flag)) return false;
   }
 }
 

@@ -197,6 +197,12 @@ int b200_dense_w4(const void* X, int64_t ldx, int x_dtype, const float* x_scales
   return done(dense_w4(p, status, static_cast<cudaStream_t>(stream)), "dense_w4");
 }
 
+int b200_debug_w4_expire(int64_t limit_ns) {
+  if (limit_ns < 0) return bad("limit_ns must not be negative");
+  w4_expire(limit_ns);
+  return report_ok();
+}
+
 int b200_token_logprobs(const void* logits, int64_t ld, int dtype, int64_t T, int64_t V,
                         const int32_t* tokens, float* logprobs, float* entropy, int top,
                         float* top_logprobs, int32_t* top_tokens, void* stream) {

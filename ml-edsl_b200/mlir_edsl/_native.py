@@ -50,7 +50,7 @@ EXPORTED_SYMBOLS = [
     "b200_memref_bias_add_f32", "b200_memref_bias_relu_f32", "b200_memref_relu_f32",
     "b200_rms_norm", "b200_w4_bytes", "b200_w4_quantize", "b200_w4_pack", "b200_w4_dequantize",
     "b200_dense_w4", "b200_token_logprobs", "b200_weights_register_w4", "b200_weights_w4",
-    "b200_weights_release_w4",
+    "b200_weights_release_w4", "b200_debug_w4_expire",
 ]
 
 _lib = None
@@ -145,6 +145,7 @@ def _declare(lib):
         "b200_weights_register_w4": ([vp, i64, i64, i64, i32, c.c_uint64], i32),
         "b200_weights_w4": ([vp, c.POINTER(vp)], i32),
         "b200_weights_release_w4": ([vp], i32),
+        "b200_debug_w4_expire": ([i64], i32),
         "b200_token_logprobs": ([vp, i64, i32, i64, i64, vp, vp, vp, i32, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():

@@ -17,9 +17,13 @@ The operators around the dense layers of a network whose weights are kept in
 
 Rows are the last dimension: tensors of any number of dimensions whose leading
 ones can be viewed as one, with contiguous rows. Wrong types raise TypeError,
-wrong shapes, strides or devices ValueError. Nothing here synchronises or
-keeps scratch, so calls can be captured into CUDA graphs. There is no backward
+wrong shapes, strides or devices ValueError. Nothing here (but check) synchronises
+or keeps scratch, so calls can be captured into CUDA graphs. There is no backward
 pass: tensors that require gradients are refused while gradients are enabled.
+
+dense_w4 of more than 8 rows (f32: 2) bounds the waits inside its kernel. One that
+runs out, which no sound GPU lets happen, makes the results around it NaN;
+check() raises it.
 """
 import os
 from importlib.machinery import ExtensionFileLoader
@@ -118,6 +122,14 @@ def dense_w4(x, w: W4Weights, bias=None, *, act: int = ACT_NONE, alpha: float = 
     if not isinstance(w, W4Weights):
         raise TypeError(f"w: expected W4Weights, got {type(w).__name__}")
     return _calls.dense_w4(x, w._packed, bias, act, alpha, x_scales, x_group, out_dtype, out)
+
+
+def check(device=None):
+    """Waits for the current stream of `device` (the current one where None) and
+    raises B200Error if a kernel there gave up a wait since the last check."""
+    with torch.cuda.device(device):
+        stream = torch.cuda.current_stream().cuda_stream
+        _native.check(_native.lib().b200_stream_sync(stream))
 
 
 class TokenLogprobs(NamedTuple):

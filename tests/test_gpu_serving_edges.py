@@ -119,3 +119,26 @@ def test_rms_norm_of_tiny_rows_and_eps(cuda, N):
     synced()
     want = norm_formula(x, eps)
     assert ((y.double() - want).abs() <= half_step(want, F32) + NORM_F32 * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, E4M3])
+@pytest.mark.parametrize("M,K,group", [(9, 64, 64), (40, 4096, 128), (100, 1000, 32)])
+def test_dense_w4_waits_that_run_out(cuda, dtype, M, K, group):
+    """Waits for products that never report their end give up after 1 ms: the
+    result is NaN throughout, check() raises once, the next call is right."""
+    w = serving.quantize_w4(rand(cuda, 1, K, 300), group=group)
+    x = rand(cuda, 2, M, K).to(dtype)
+    want = serving.dense_w4(x, w, act=1, out_dtype=BF16)
+    serving.check()
+    expire = _native.lib().b200_debug_w4_expire
+    _native.check(expire(1_000_000))
+    try:
+        y = serving.dense_w4(x, w, act=1, out_dtype=BF16)
+        with pytest.raises(_native.B200Error, match="bounded wait") as e:
+            serving.check()
+    finally:
+        _native.check(expire(0))
+    assert e.value.code == 5 and torch.isnan(y).all()
+    serving.check(cuda)
+    assert torch.equal(serving.dense_w4(x, w, act=1, out_dtype=BF16), want)
+    serving.check()
