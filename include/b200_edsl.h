@@ -359,7 +359,8 @@ int b200_rms_norm(const void* X, int64_t ldx, const void* R, int64_t ldr, int dt
  * and group 32 or a multiple of 64 (the last group of K may be shorter).
  * b200_w4_quantize makes codes and scales of f32 weights:
  * scale = max|w| / 7 over the group, rounded to the scales' type (s_dtype:
- * f32, bf16 or f16), code = round(w / scale) + 8.
+ * f32, bf16 or f16), code = round(w / scale) + 8; the scale is NaN where the
+ * group holds an infinity or NaN.
  * b200_w4_pack lays codes, scales and zeros (or NULL) out as b200_dense_w4
  * reads them, into b200_w4_bytes(...) bytes at a 16-byte aligned address;
  * b200_w4_dequantize gives the f32 matrix of packed weights, for example for

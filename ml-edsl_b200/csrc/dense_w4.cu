@@ -134,8 +134,9 @@ __global__ void w4_pack_columns_kernel(const void* __restrict__ in, int64_t ldi,
 }
 
 // Codes and scales of W: s = max|w| / 7 over a group of one column, rounded
-// to the scales' type; q = round(w / s) + 8 with ties to even. A thread has
-// one column of one group.
+// to the scales' type; q = round(w / s) + 8 with ties to even. A group that holds
+// an infinity or NaN has a NaN for a scale, so that it shows in every product. A
+// thread has one column of one group.
 __global__ void w4_quantize_kernel(const float* __restrict__ W, int64_t ldw, int64_t K, int64_t N,
                                    int group, int64_t groups, uint8_t* __restrict__ codes,
                                    int64_t ldc, void* __restrict__ scales, int64_t lds,
@@ -146,8 +147,13 @@ __global__ void w4_quantize_kernel(const float* __restrict__ W, int64_t ldw, int
     const int64_t g = i / N, n = i - g * N;
     const int64_t k0 = g * group, k1 = min(K, k0 + group);
     float most = 0.0f;
-    for (int64_t k = k0; k < k1; ++k) most = fmaxf(most, fabsf(W[k * ldw + n]));
-    float s = most / 7.0f;
+    bool finite = true;
+    for (int64_t k = k0; k < k1; ++k) {
+      const float a = fabsf(W[k * ldw + n]);
+      finite &= a < __int_as_float(0x7f800000);
+      most = fmaxf(most, a);
+    }
+    float s = finite ? most / 7.0f : __int_as_float(0x7fc00000);
     if (s_dtype == kBF16) {
       const bf16 r = __float2bfloat16_rn(s);
       static_cast<bf16*>(scales)[g * lds + n] = r;

@@ -103,7 +103,9 @@ def pack_w4(codes, scales, zeros=None, *, group: int = 128) -> W4Weights:
 
 def quantize_w4(W, *, group: int = 128, scale_dtype=torch.float32) -> W4Weights:
     """4-bit weights of the f32 matrix W [K, N]: scale = max|W| / 7 over each
-    group of K and column (rounded to scale_dtype), code = round(W / scale) + 8."""
+    group of K and column (rounded to scale_dtype), code = round(W / scale) + 8. A
+    group that holds an infinity or NaN, or whose scale is past scale_dtype's
+    range, becomes NaN."""
     codes, scales = _calls.quantize_w4(W, group, scale_dtype)
     return pack_w4(codes, scales, group=group)
 

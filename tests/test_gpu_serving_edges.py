@@ -142,3 +142,18 @@ def test_dense_w4_waits_that_run_out(cuda, dtype, M, K, group):
     serving.check(cuda)
     assert torch.equal(serving.dense_w4(x, w, act=1, out_dtype=BF16), want)
     serving.check()
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("value", [NAN, INF, -INF])
+def test_quantize_of_weights_that_are_not_finite(cuda, scale_dtype, value):
+    """A weight that is no number shows: its group of its column is NaN, and
+    nothing else changes."""
+    W = rand(cuda, 1, 200, 40)
+    clean = serving.quantize_w4(W, group=64, scale_dtype=scale_dtype).dequantize()
+    W[70, 3] = value
+    got = serving.quantize_w4(W, group=64, scale_dtype=scale_dtype).dequantize()
+    synced()
+    assert torch.isnan(got[64:128, 3]).all()
+    got[64:128, 3] = clean[64:128, 3]
+    assert torch.equal(got, clean)
