@@ -342,8 +342,8 @@ int b200_host_free(void* ptr);
 /* Root-mean-square norm of the rows of X[M,N]:
  *   h = X + R;  y = h / sqrt(mean(h^2) + eps) * w
  * X, R (or NULL) and H (or NULL: not stored) are of type `dtype`; w[N] (or
- * NULL: 1) is of that type or f32. H may be X or R itself (same address and
- * pitch). y is computed in f32 from the f32 sum and rounded once into Y:
+ * NULL: 1) is of that type or f32. H, and a Y of X's type, may be X or R itself
+ * (same address and pitch; not both the same one). y is computed in f32 from the f32 sum and rounded once into Y:
  * of X's type (y_dtype == dtype, scales NULL), or e4m3 codes
  * (y_dtype B200_E4M3) with scales: the value is code * scale, and
  * scale = max|y| / 448 over the row (group 0: scales[m * ld_scales]) or over

@@ -132,6 +132,49 @@ Rows rows(const Tensor& t, const char* name) {
   return {m, n, std::max(ld, n)};
 }
 
+// The bytes of a tensor's rows: `rows` of them, `n` bytes each, `ld` apart.
+struct Memory {
+  const char* at;
+  int64_t m, n, ld;
+  const char* end() const { return at + (m - 1) * ld + n; }
+};
+Memory memory(const Tensor& t, const Rows& r) {
+  const int64_t size = (int64_t)t.element_size();
+  return {static_cast<const char*>(t.const_data_ptr()), r.n ? r.m : 0, r.n * size, r.ld * size};
+}
+Memory memory(const Tensor& t, const char* name) { return memory(t, rows(t, name)); }
+
+bool same(const Memory& a, const Memory& b) {
+  return a.at == b.at && a.m == b.m && a.n == b.n && (a.m == 1 || a.ld == b.ld);
+}
+
+// Whether two sets of rows share a byte. Rows of one pitch may lie side by side
+// in one buffer; of other pitches, both are gone through in the order of their
+// addresses.
+bool overlap(const Memory& a, const Memory& b) {
+  if (a.m == 0 || b.m == 0 || a.end() <= b.at || b.end() <= a.at) return false;
+  if (a.ld == b.ld) {
+    // a row of b starts d bytes behind one of a, and ld - d before the next (the
+    // ends overlap, so at least one of the two is there)
+    const int64_t d = ((b.at - a.at) % a.ld + a.ld) % a.ld;
+    return d < a.n || a.ld - d < b.n;
+  }
+  for (int64_t i = 0, j = 0; i < a.m && j < b.m;) {
+    const char *p = a.at + i * a.ld, *q = b.at + j * b.ld;
+    if (p < q + b.n && q < p + a.n) return true;
+    if (p < q) ++i;
+    else ++j;
+  }
+  return false;
+}
+
+// Refuses an output that shares memory with `b`, unless it may take its place.
+void check_apart(const Memory& out, const char* name, const Memory& b, const char* other,
+                 bool in_place = false) {
+  if (overlap(out, b) && !(in_place && same(out, b)))
+    value_error(std::string(name) + ": overlaps " + other);
+}
+
 const void* vector(PyObject* o, int64_t n, const char* name, Types types,
                    const c10::Device& device, int* code) {
   const Tensor& t = tensor(o, name, types, &device);
@@ -245,20 +288,34 @@ PyObject* rms_norm(PyObject* const* a) {
   const void* r = nullptr;
   Tensor h;
   int64_t ldr = 0, ldh = 0;
+  const Memory mx = memory(x, rx);
+  Memory mr{}, mh{};
+  auto apart = [&](const Memory& out, const char* name, bool in_place) {
+    check_apart(out, name, mx, "x", in_place);
+    if (r) check_apart(out, name, mr, "residual", in_place);
+    if (w) check_apart(out, name, memory(THPVariable_Unpack(a[1]), "weight"), "weight");
+  };
   if (a[2] != Py_None) {
     const Tensor& res = tensor(a[2], "residual", {type}, &device);
     if (res.sizes() != x.sizes())
       value_error("residual: expected shape " + text_of(x.sizes()) + ", got " +
                   text_of(res.sizes()));
+    mr = memory(res, "residual");
     ldr = rows(res, "residual").ld;
     r = res.const_data_ptr();
     h = output(a[7], x.sizes(), type, device, "residual_out");
     ldh = rows(h, "residual_out").ld;
+    if (a[7] != Py_None) apart(mh = memory(h, "residual_out"), "residual_out", true);
   } else if (a[7] != Py_None) {
     value_error("residual_out: given without a residual");
   }
   Tensor y = output(a[6], x.sizes(), quant ? ScalarType::Float8_e4m3fn : type, device, "out");
   const int64_t ldy = rows(y, "out").ld;
+  if (a[6] != Py_None) {
+    const Memory my = memory(y, "out");
+    apart(my, "out", !quant);
+    check_apart(my, "out", mh, "residual_out");
+  }
   Tensor s;
   int64_t lds = 0;
   if (quant) {
@@ -415,6 +472,13 @@ PyObject* dense_w4(PyObject* const* a) {
   if (a[2] != Py_None) b = vector(a[2], w.N, "bias", PLAIN_TYPES, device, &b_code);
   Tensor y = output(a[8], lead_and(x, w.N), type, device, "out");
   const int64_t ldy = rows(y, "out").ld;
+  if (a[8] != Py_None) {
+    const Memory my = memory(y, "out");
+    check_apart(my, "out", memory(x, r), "x");
+    check_apart(my, "out", memory(*w.buffer, "w"), "w");
+    if (b) check_apart(my, "out", memory(THPVariable_Unpack(a[2]), "bias"), "bias");
+    if (xs) check_apart(my, "out", memory(THPVariable_Unpack(a[5]), "x_scales"), "x_scales");
+  }
   call(device, [&](void* stream) {
     return b200_dense_w4(x.const_data_ptr(), r.ld, code_of(x.scalar_type()), xs, lds, (int)x_group,
                          w.buffer->const_data_ptr(), w.s_code, w.has_zeros, w.group, b, b_code,
@@ -465,6 +529,14 @@ PyObject* rows_of(PyObject* const* a) {
   return Py_BuildValue("(LLL)", (long long)r.m, (long long)r.n, (long long)r.ld);
 }
 
+// two tensors on any device -> whether they share memory
+PyObject* overlap_of(PyObject* const* a) {
+  for (int i = 0; i < 2; ++i)
+    if (!THPVariable_Check(a[i])) type_error("expected a torch tensor");
+  return PyBool_FromLong(overlap(memory(THPVariable_Unpack(a[0]), "tensor"),
+                                 memory(THPVariable_Unpack(a[1]), "tensor")));
+}
+
 // the exceptions of failed calls and of allocations
 PyObject* set_errors(PyObject* const* a) {
   Py_INCREF(a[0]);
@@ -509,7 +581,8 @@ PyMethodDef g_methods[] = {
     method<rms_norm, 8>("rms_norm"),           method<pack_w4, 4>("pack_w4"),
     method<quantize_w4, 3>("quantize_w4"),     method<dequantize_w4, 1>("dequantize_w4"),
     method<dense_w4, 9>("dense_w4"),           method<token_logprobs, 3>("token_logprobs"),
-    method<rows_of, 1>("rows_of"),             method<set_errors, 2>("set_errors"),
+    method<rows_of, 1>("rows_of"),             method<overlap_of, 2>("overlap_of"),
+    method<set_errors, 2>("set_errors"),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "b200torch", nullptr, -1, g_methods,

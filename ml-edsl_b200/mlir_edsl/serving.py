@@ -62,9 +62,10 @@ def rms_norm(x, weight=None, *, residual=None, eps: float = 1e-6, quant: Optiona
     Returns y in x's type or, with quant="e4m3", the codes (torch.float8_e4m3fn)
     and their f32 scales, one for each row (group 0) or each `group` (32, 64 or
     128) columns: y = codes * scales. With a residual, h in x's type comes
-    last: y, h or codes, scales, h. h goes to `residual_out` (which may be x or
-    residual itself) and y or the codes to `out` where these are given. y is
-    computed from h before its rounding and rounded once."""
+    last: y, h or codes, scales, h. h goes to `residual_out` and y or the codes to
+    `out` where these are given; h and y may take the place of x or of residual,
+    but outputs that overlap anything else are refused. y is computed from h
+    before its rounding and rounded once."""
     return _calls.rms_norm(x, weight, residual, eps, quant, group, out, residual_out)
 
 
@@ -120,7 +121,8 @@ def dense_w4(x, w: W4Weights, bias=None, *, act: int = ACT_NONE, alpha: float = 
     x: f32, bf16, f16, or e4m3 codes with x_scales [..., 1] (x_group 0) or
     [..., ceil(K / x_group)] as rms_norm gives them. bias: [N], f32, bf16 or
     f16. The result has x's type, bf16 for e4m3, or out_dtype (f32, bf16,
-    f16). Products are exact, sums run in f32, the result is rounded once."""
+    f16); it goes to `out` where that is given, which must not overlap an input.
+    Products are exact, sums run in f32, the result is rounded once."""
     if not isinstance(w, W4Weights):
         raise TypeError(f"w: expected W4Weights, got {type(w).__name__}")
     return _calls.dense_w4(x, w._packed, bias, act, alpha, x_scales, x_group, out_dtype, out)

@@ -157,3 +157,55 @@ def test_quantize_of_weights_that_are_not_finite(cuda, scale_dtype, value):
     assert torch.isnan(got[64:128, 3]).all()
     got[64:128, 3] = clean[64:128, 3]
     assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("M,N", [(1, 1), (5, 4096), (300, 1001), (40, 8200), (3, 20001), (2, 100003)])
+def test_rms_norm_over_its_inputs(cuda, dtype, M, N):
+    """The result may take the place of x or of the residual."""
+    x, r = (rand(cuda, 1, M, N) * 2).to(dtype), rand(cuda, 2, M, N).to(dtype)
+    want = serving.rms_norm(x)
+    want_y, want_h = serving.rms_norm(x, residual=r)
+    a = x.clone()
+    assert serving.rms_norm(a, out=a) is a
+    b, c = x.clone(), r.clone()
+    serving.rms_norm(b, residual=c, out=b, residual_out=c)
+    d, e = x.clone(), r.clone()
+    _, h = serving.rms_norm(d, residual=e, out=e)
+    synced()
+    assert torch.equal(a, want)
+    assert torch.equal(b, want_y) and torch.equal(c, want_h)
+    assert torch.equal(e, want_y) and torch.equal(h, want_h)
+
+
+def test_outputs_that_overlap_are_refused(cuda):
+    buf = rand(cuda, 1, 8, 512)
+    x, r = buf[1:5, :128], buf[1:5, 128:256]
+    side = buf[1:5, 256:384]
+    serving.rms_norm(x, residual=r, out=side)  # columns of one buffer, side by side
+    weight = rand(cuda, 2, 1024)[:128]
+    for kw in (dict(out=buf[2:6, :128]), dict(out=buf[1:5, 64:192]),
+               dict(out=side, residual_out=side), dict(residual_out=buf[0:4, 128:256])):
+        with pytest.raises(ValueError, match="overlap"):
+            serving.rms_norm(x, residual=r, **kw)
+    line = rand(cuda, 2, 128)
+    with pytest.raises(ValueError, match="overlap"):
+        serving.rms_norm(x[:1], line, out=line[None])
+    with pytest.raises(ValueError, match="overlap"):
+        serving.rms_norm(rand(cuda, 2, 1, 128), weight, quant="e4m3",
+                         out=weight.view(torch.float8_e4m3fn)[None, :128])
+    w = serving.quantize_w4(rand(cuda, 3, 128, 128), group=64)
+    serving.dense_w4(x, w, out=side)
+    bias = rand(cuda, 4, 4, 128)
+    with pytest.raises(ValueError, match="overlap"):
+        serving.dense_w4(x, w, out=x)
+    with pytest.raises(ValueError, match="overlap"):
+        serving.dense_w4(x, w, out=buf[3:7, 100:228])
+    with pytest.raises(ValueError, match="overlap"):
+        serving.dense_w4(x, w, bias[2], out=bias)
+    with pytest.raises(ValueError, match="overlap"):
+        serving.dense_w4(x[:1], w, out=w.buffer.view(F32)[None, :128])
+    s = torch.ones(4, 128, device=cuda)
+    with pytest.raises(ValueError, match="overlap"):
+        serving.dense_w4(x.to(E4M3), w, x_scales=s[:, :2], x_group=64, out=s)
+    synced()
