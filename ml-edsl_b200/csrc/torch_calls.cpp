@@ -201,6 +201,11 @@ Tensor output(PyObject* o, at::IntArrayRef shape, ScalarType type, const c10::De
   return t;
 }
 
+// A given output has new contents: backward passes that kept it have to notice.
+void changed(PyObject* o, const Tensor& t) {
+  if (o != Py_None && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::DimVector lead(const Tensor& t) {
   return at::DimVector(t.sizes().begin(), t.sizes().end() - 1);
 }
@@ -329,6 +334,8 @@ PyObject* rms_norm(PyObject* const* a) {
                          quant ? static_cast<float*>(s.data_ptr()) : nullptr, lds, (int)group,
                          rx.m, rx.n, stream);
   });
+  changed(a[6], y);
+  changed(a[7], h);
   if (quant) return h.defined() ? wrap_all({y, s, h}) : wrap_all({y, s});
   return h.defined() ? wrap_all({y, h}) : wrap(y);
 }
@@ -484,6 +491,7 @@ PyObject* dense_w4(PyObject* const* a) {
                          w.buffer->const_data_ptr(), w.s_code, w.has_zeros, w.group, b, b_code,
                          y.data_ptr(), ldy, code_of(type), r.m, w.N, w.K, act, alpha, stream);
   });
+  changed(a[8], y);
   return wrap(y);
 }
 

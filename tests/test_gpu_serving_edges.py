@@ -209,3 +209,28 @@ def test_outputs_that_overlap_are_refused(cuda):
     with pytest.raises(ValueError, match="overlap"):
         serving.dense_w4(x.to(E4M3), w, x_scales=s[:, :2], x_group=64, out=s)
     synced()
+
+
+def test_outputs_count_as_changed(cuda):
+    """A tensor that a backward pass needs and that a call overwrites is noticed."""
+    x, r = rand(cuda, 1, 4, 64), rand(cuda, 2, 4, 64)
+    out, h = torch.ones_like(x), torch.ones_like(x)
+    leaf = torch.ones(4, 64, device=cuda, requires_grad=True)
+    loss = (leaf * out).sum()
+    before = out._version, h._version, x._version
+    serving.rms_norm(x, residual=r, out=out, residual_out=h)
+    assert (out._version, h._version, x._version) == (before[0] + 1, before[1] + 1, before[2])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    w = serving.quantize_w4(rand(cuda, 3, 64, 64), group=64)
+    serving.dense_w4(x, w, out=out)
+    assert out._version == before[0] + 2
+    serving.rms_norm(x, residual=r, residual_out=r)  # one change, not two
+    assert r._version == 1
+    with pytest.raises(ValueError):
+        serving.dense_w4(x, w, out=h[:2])
+    assert h._version == before[1] + 1  # a refused call changes nothing
+    with torch.inference_mode():
+        kept = torch.empty_like(x)
+    serving.rms_norm(x, out=kept)  # has no version
+    synced()
