@@ -9,6 +9,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -99,6 +100,10 @@ const Tensor& tensor(PyObject* o, const char* name, Types types,
     value_error(std::string(name) +
                 ": requires a gradient, and this operator has no backward pass (use "
                 "torch.no_grad())");
+  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    value_error(std::string(name) +
+                ": has a tangent, and this operator has no forward gradient (use "
+                "torch.autograd.forward_ad.unpack_dual)");
   return t;
 }
 

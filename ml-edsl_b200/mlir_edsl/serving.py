@@ -19,7 +19,8 @@ Rows are the last dimension: tensors of any number of dimensions whose leading
 ones can be viewed as one, with contiguous rows. Wrong types raise TypeError,
 wrong shapes, strides or devices ValueError. Nothing here (but check) synchronises
 or keeps scratch, so calls can be captured into CUDA graphs. There is no backward
-pass: tensors that require gradients are refused while gradients are enabled.
+pass: tensors that require gradients are refused while gradients are enabled, and
+tensors with tangents of forward differentiation always.
 
 dense_w4 of more than 8 rows (f32: 2) bounds the waits inside its kernel. One that
 runs out, which no sound GPU lets happen, makes the results around it NaN;

@@ -234,3 +234,21 @@ def test_outputs_count_as_changed(cuda):
         kept = torch.empty_like(x)
     serving.rms_norm(x, out=kept)  # has no version
     synced()
+
+
+def test_forward_gradients_are_refused(cuda):
+    import torch.autograd.forward_ad as forward
+    x = rand(cuda, 1, 2, 64)
+    w = serving.quantize_w4(rand(cuda, 2, 64, 64), group=64)
+    with forward.dual_level():
+        dual = forward.make_dual(x, torch.ones_like(x))
+        for call in (lambda: serving.rms_norm(dual), lambda: serving.dense_w4(dual, w),
+                     lambda: serving.token_logprobs(dual), lambda: serving.quantize_w4(dual),
+                     lambda: serving.rms_norm(x, dual[0]),
+                     lambda: serving.rms_norm(x, residual=dual)):
+            with pytest.raises(ValueError, match="forward"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="forward"):
+                call()
+        serving.rms_norm(forward.unpack_dual(dual).primal)
+    synced()
