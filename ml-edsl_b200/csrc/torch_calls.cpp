@@ -93,6 +93,9 @@ const Tensor& tensor(PyObject* o, const char* name, Types types,
   check_type(t.scalar_type(), name, types);
   if (!t.is_cuda() || t.layout() != c10::kStrided)
     value_error(std::string(name) + ": expected a CUDA tensor, got one on " + t.device().str());
+  if (t.is_neg())
+    value_error(std::string(name) +
+                ": stands for the negative of its memory (use torch.resolve_neg)");
   if (device && t.device() != *device)
     value_error(std::string(name) + ": on " + t.device().str() + ", but the call runs on " +
                 device->str());

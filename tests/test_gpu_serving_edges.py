@@ -252,3 +252,18 @@ def test_forward_gradients_are_refused(cuda):
                 call()
         serving.rms_norm(forward.unpack_dual(dual).primal)
     synced()
+
+
+def test_negated_views_are_refused(cuda):
+    """A view that stands for the negative of its memory (the imaginary part of a
+    conjugate, for example)."""
+    part = torch.complex(rand(cuda, 1, 3, 1), rand(cuda, 2, 3, 1)).conj().imag
+    with pytest.raises(ValueError, match="resolve_neg"):
+        serving.rms_norm(part)
+    x = rand(cuda, 3, 3, 64)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        serving.token_logprobs(torch._neg_view(x))
+    with pytest.raises(ValueError, match="resolve_neg"):
+        serving.rms_norm(x, out=torch._neg_view(x.clone()))
+    serving.rms_norm(part.resolve_neg())
+    synced()
