@@ -71,8 +71,9 @@ int b200_rms_norm(const void* X, int64_t ldx, const void* R, int64_t ldr, int dt
   if (group != 0 && group != 32 && group != 64 && group != 128)
     return bad("group must be 0 (a row), 32, 64 or 128");
   if (group != 0 && y_dtype != kE4M3) return bad("only an e4m3 Y has groups");
-  if (M == 0 || N == 0) return report_ok();
-  if (!X || !Y || ldx < N || ldy < N || (R && ldr < N) || (H && ldh < N))
+  // rows without columns have a scale each all the same, of 1
+  if (M == 0 || (N == 0 && (!scales || group != 0))) return report_ok();
+  if ((N > 0 && (!X || !Y)) || ldx < N || ldy < N || (R && ldr < N) || (H && ldh < N))
     return bad("null buffer or pitch < N");
   if (scales && ld_scales < (group ? (N + group - 1) / group : 1))
     return bad("pitch of scales < number of groups");

@@ -267,3 +267,15 @@ def test_negated_views_are_refused(cuda):
         serving.rms_norm(x, out=torch._neg_view(x.clone()))
     serving.rms_norm(part.resolve_neg())
     synced()
+
+
+def test_rms_norm_scales_of_rows_without_columns(cuda):
+    junk = torch.full((64,), 7.0, device=cuda)
+    del junk  # the allocator hands its memory to the scales
+    x = torch.empty(5, 0, device=cuda)
+    q, s = serving.rms_norm(x, quant="e4m3")
+    synced()
+    assert q.shape == (5, 0) and (s == 1).all() and s.shape == (5, 1)
+    q, s = serving.rms_norm(x, torch.empty(0, device=cuda), quant="e4m3", group=32)
+    synced()
+    assert q.shape == (5, 0) and s.shape == (5, 0)
