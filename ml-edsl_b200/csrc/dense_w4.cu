@@ -30,6 +30,7 @@
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <cstdint>
+#include "device_facts.h"
 #include "w4.cuh"
 
 namespace cg = cooperative_groups;
@@ -60,10 +61,11 @@ Capacity::Capacity(const void* kernel, int threads, int smem) {
     at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    int clusters = 0;
-    const bool known = cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess;
-    if (!known) cudaGetLastError();  // the next launch is not to report it
-    ctas[l] = known && clusters > 0 ? (int64_t)clusters << l : l == 0 ? 148 : 0;
+    const int clusters = ask_or(
+        l == 0 ? 148 : 0,
+        [&](int* n) { return cudaOccupancyMaxActiveClusters(n, kernel, &cfg) == cudaSuccess; },
+        [] { cudaGetLastError(); });
+    ctas[l] = (int64_t)clusters << l;
   }
 }
 

@@ -1,5 +1,7 @@
 """The serving operators at their edges, as far as no GPU is needed."""
+import os
 import random
+import subprocess
 
 import torch
 
@@ -37,3 +39,35 @@ def test_overlap_of_rows():
     assert not overlap(cols[:, 4:8], cols[:, 8:32]) and overlap(cols[:, 4:9], cols[:, 8:32])
     assert overlap(cols[:, 30:], cols.view(3, 64)[:, 62:])
     assert not overlap(cols[:, 30:], cols.view(3, 64)[:, :30])
+
+
+def _run_cpp(tmp_path, body):
+    """Compiles and runs a program around csrc/device_facts.h; its main is `body`."""
+    csrc = os.path.join(os.path.dirname(_native.__file__), "..", "csrc")
+    src, exe = tmp_path / "facts.cpp", tmp_path / "facts"
+    src.write_text('#include "device_facts.h"\n#include <cassert>\n#include <thread>\n'
+                   "#include <vector>\nint main() {\n" + body + "\nreturn 0;\n}\n")
+    subprocess.run(["g++", "-std=c++17", "-UNDEBUG", "-I", csrc, str(src), "-o", str(exe),
+                    "-lpthread"], check=True)
+    subprocess.run([str(exe)], check=True, timeout=60)
+
+
+def test_a_failing_query_leaves_no_error_behind(tmp_path):
+    _run_cpp(tmp_path, """
+      int errors = 0;  // what the next check would find
+      auto forget = [&] { errors = 0; };
+      auto fails = [&](int* n) { *n = 7; ++errors; return false; };
+      assert(b200::ask_or(3, fails, forget) == 3 && errors == 0);
+      auto gives = [](int value) { return [=](int* n) { *n = value; return true; }; };
+      errors = 5;  // an error that was there before is the caller's
+      assert(b200::ask_or(3, gives(4), forget) == 4 && errors == 5);
+      assert(b200::ask_or(3, gives(0), forget) == 3 && errors == 5);""")
+
+
+def test_queries_go_through_it():
+    """No occupancy query but those that ask_or makes."""
+    csrc = os.path.join(os.path.dirname(_native.__file__), "..", "csrc")
+    for name in os.listdir(csrc):
+        text = open(os.path.join(csrc, name)).read()
+        for part in text.split("cudaOccupancy")[:-1]:
+            assert "ask_or(" in part[-200:], name
