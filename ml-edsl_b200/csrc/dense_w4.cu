@@ -30,17 +30,17 @@
 #include <cuda_runtime.h>
 #include <algorithm>
 #include <cstdint>
-#include "device_facts.h"
 #include "w4.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace b200 {
 
-cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed) {
+cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed, int* device) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (device) *device = dev;
   const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
   if (allowed.load(std::memory_order_relaxed) & bit) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
@@ -48,7 +48,8 @@ cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed) {
   return e;
 }
 
-Capacity::Capacity(const void* kernel, int threads, int smem) {
+Capacity capacity_of(const void* kernel, int threads, int smem) {
+  Capacity c;
   for (int l = 0; l < 4; ++l) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(8u * 148);
@@ -65,8 +66,9 @@ Capacity::Capacity(const void* kernel, int threads, int smem) {
         l == 0 ? 148 : 0,
         [&](int* n) { return cudaOccupancyMaxActiveClusters(n, kernel, &cfg) == cudaSuccess; },
         [] { cudaGetLastError(); });
-    ctas[l] = (int64_t)clusters << l;
+    c.ctas[l] = (int64_t)clusters << l;
   }
+  return c;
 }
 
 int choose_cluster(const Capacity& capacity, int64_t tiles, int64_t kblocks, int warps, int fixed) {
@@ -517,9 +519,13 @@ int launch_few(W4Params p, cudaStream_t st) {
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
   if (chunks > 65535) return kErrTooLarge;
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
+  int dev = 0;
+  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed, &dev);
   if (e0 != cudaSuccess) return launch_result(e0);
-  static const Capacity capacity(reinterpret_cast<const void*>(kernel), kFewWarps * 32, kFewShared);
+  static PerDevice<Capacity> capacities;
+  const Capacity capacity = capacities.of(dev, [&] {
+    return capacity_of(reinterpret_cast<const void*>(kernel), kFewWarps * 32, kFewShared);
+  });
   const int best = choose_cluster(capacity, tiles * chunks, p.kblocks, kFewWarps, 4);
   const int C = 1 << best;
   p.log_cluster = best;

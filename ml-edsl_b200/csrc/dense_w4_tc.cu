@@ -545,9 +545,13 @@ int launch(W4Params p, int* status, cudaStream_t st) {
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
   if (chunks > 65535) return kErrTooLarge;
   static std::atomic<uint64_t> allowed{0};
-  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed);
+  int dev = 0;
+  const cudaError_t e0 = allow_shared(reinterpret_cast<const void*>(kernel), allowed, &dev);
   if (e0 != cudaSuccess) return launch_result(e0);
-  static const Capacity capacity(reinterpret_cast<const void*>(kernel), S::kThreads, kMaxShared);
+  static PerDevice<Capacity> capacities;
+  const Capacity capacity = capacities.of(dev, [&] {
+    return capacity_of(reinterpret_cast<const void*>(kernel), S::kThreads, kMaxShared);
+  });
   const int best = choose_cluster(capacity, tiles * chunks, p.kblocks, 1, 8);
   const int C = 1 << best;
   p.log_cluster = best;

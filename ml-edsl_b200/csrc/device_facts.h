@@ -1,8 +1,32 @@
 // What the host asks the driver about a device and a kernel before it launches.
 // No CUDA in here: the queries are the callers'.
 #pragma once
+#include <mutex>
 
 namespace b200 {
+
+// A value for each device, made when it is first asked for there; once, also when
+// several threads ask at the same time. Devices differ, and what one gives must
+// not decide how another one runs.
+template <class T>
+class PerDevice {
+ public:
+  template <class Make>
+  T of(int device, Make make) {
+    if (device < 0 || device >= kDevices) return make();
+    Slot& s = slots_[device];
+    std::call_once(s.once, [&] { s.value = make(); });
+    return s.value;
+  }
+
+ private:
+  static constexpr int kDevices = 64;
+  struct Slot {
+    std::once_flag once;
+    T value{};
+  };
+  Slot slots_[kDevices];
+};
 
 // What `ask(&n)` gives (true: the query went well), or `otherwise` where it fails
 // or gives nothing. `forget` takes the error of a failing query back, so that the

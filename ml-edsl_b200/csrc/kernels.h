@@ -29,8 +29,9 @@ void count_launch();
 constexpr int kMaxShared = 200 * 1024;
 
 // Lets `kernel` use kMaxShared of dynamic shared memory on the current device.
-// `allowed`: one bit a device that has been told.
-cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed);
+// `allowed`: one bit a device that has been told. `device`: which one it is.
+cudaError_t allow_shared(const void* kernel, std::atomic<uint64_t>& allowed,
+                         int* device = nullptr);
 
 // Records an error for b200_last_error()/b200_last_status() on this thread
 // and returns `code`; report_ok() records success and returns kOk.

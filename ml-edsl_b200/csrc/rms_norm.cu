@@ -568,12 +568,19 @@ cudaError_t launch(const RmsNormArgs& p, cudaStream_t st) {
   constexpr int ROWS = TPR < 128 ? 128 / TPR : 1, THREADS = TPR < 128 ? 128 : TPR;
   auto kernel = rms_norm_kernel<T, TPR, E, HOW>;
   // as many CTAs as fit, each with the rows that fall to it
-  static const int per_sm = ask_or(
-      1,
-      [&](int* n) {
-        return cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, kernel, THREADS, 0) == cudaSuccess;
-      },
-      [] { cudaGetLastError(); });
+  static PerDevice<int> resident;
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const int per_sm = resident.of(dev, [&] {
+    return ask_or(
+        1,
+        [&](int* n) {
+          return cudaOccupancyMaxActiveBlocksPerMultiprocessor(n, kernel, THREADS, 0) ==
+                 cudaSuccess;
+        },
+        [] { cudaGetLastError(); });
+  });
   const int64_t grid = std::min<int64_t>((p.M + ROWS - 1) / ROWS, (int64_t)148 * per_sm);
   return launch_kernel(kernel, (unsigned)grid, THREADS, 0, p, st);
 }

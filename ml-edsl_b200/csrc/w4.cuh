@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include <cstdint>
+#include "device_facts.h"
 #include "dtype.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
@@ -254,12 +255,12 @@ __device__ __forceinline__ void prefetch_strip(const W4Params& p, int64_t strip,
   if (p.zeros) prefetch_l2_bulk(p.zeros + at, (uint32_t)elems);
 }
 
-// How many CTAs of `kernel` run at once in clusters of 1, 2, 4 and 8. GPUs
-// differ in how many clusters fit, so the driver is asked, once a kernel.
+// How many CTAs of a kernel run at once in clusters of 1, 2, 4 and 8. GPUs differ
+// in how many clusters fit, so the driver is asked, once a kernel and device.
 struct Capacity {
   int64_t ctas[4];
-  Capacity(const void* kernel, int threads, int smem);
 };
+Capacity capacity_of(const void* kernel, int threads, int smem);
 
 // The log2 of the CTAs that share K, of `tiles` CTAs' work each `kblocks` long
 // that `warps` warps split: the fewest waves, each as long as a warp's blocks

@@ -45,7 +45,7 @@ def _run_cpp(tmp_path, body):
     """Compiles and runs a program around csrc/device_facts.h; its main is `body`."""
     csrc = os.path.join(os.path.dirname(_native.__file__), "..", "csrc")
     src, exe = tmp_path / "facts.cpp", tmp_path / "facts"
-    src.write_text('#include "device_facts.h"\n#include <cassert>\n#include <thread>\n'
+    src.write_text('#include "device_facts.h"\n#include <atomic>\n#include <cassert>\n#include <thread>\n'
                    "#include <vector>\nint main() {\n" + body + "\nreturn 0;\n}\n")
     subprocess.run(["g++", "-std=c++17", "-UNDEBUG", "-I", csrc, str(src), "-o", str(exe),
                     "-lpthread"], check=True)
@@ -71,3 +71,27 @@ def test_queries_go_through_it():
         text = open(os.path.join(csrc, name)).read()
         for part in text.split("cudaOccupancy")[:-1]:
             assert "ask_or(" in part[-200:], name
+
+
+def test_values_for_each_device(tmp_path):
+    _run_cpp(tmp_path, """
+      static b200::PerDevice<int> values;
+      std::atomic<int> made{0};
+      auto of = [&](int device) {
+        return values.of(device, [&] { ++made; return 10 * device + 1; });
+      };
+      std::vector<std::thread> threads;
+      for (int t = 0; t < 8; ++t)
+        threads.emplace_back([&] { for (int d = 0; d < 64; ++d) assert(of(d) == 10 * d + 1); });
+      for (auto& t : threads) t.join();
+      assert(made == 64);
+      assert(of(64) == 641 && of(64) == 641 && made == 66);  // past the table: asked each time
+      assert(of(-1) == -9);""")
+
+
+def test_nothing_about_one_device_is_kept_for_all():
+    """What is kept from a query is kept for its device."""
+    csrc = os.path.join(os.path.dirname(_native.__file__), "..", "csrc")
+    for name in ("rms_norm.cu", "dense_w4.cu", "dense_w4_tc.cu", "token_logprobs.cu"):
+        text = open(os.path.join(csrc, name)).read()
+        assert "static const " not in text, name
