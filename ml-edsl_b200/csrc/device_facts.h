@@ -1,6 +1,7 @@
 // What the host asks the driver about a device and a kernel before it launches.
 // No CUDA in here: the queries are the callers'.
 #pragma once
+#include <atomic>
 #include <mutex>
 
 namespace b200 {
@@ -15,17 +16,24 @@ class PerDevice {
   T of(int device, Make make) {
     if (device < 0 || device >= kDevices) return make();
     Slot& s = slots_[device];
-    std::call_once(s.once, [&] { s.value = make(); });
+    if (!s.made.load(std::memory_order_acquire)) {
+      std::lock_guard<std::mutex> lock(making_);
+      if (!s.made.load(std::memory_order_relaxed)) {
+        s.value = make();
+        s.made.store(true, std::memory_order_release);
+      }
+    }
     return s.value;
   }
 
  private:
   static constexpr int kDevices = 64;
   struct Slot {
-    std::once_flag once;
+    std::atomic<bool> made{false};
     T value{};
   };
   Slot slots_[kDevices];
+  std::mutex making_;
 };
 
 // What `ask(&n)` gives (true: the query went well), or `otherwise` where it fails

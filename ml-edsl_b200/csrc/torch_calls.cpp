@@ -103,7 +103,9 @@ const Tensor& tensor(PyObject* o, const char* name, Types types,
     value_error(std::string(name) +
                 ": requires a gradient, and this operator has no backward pass (use "
                 "torch.no_grad())");
-  if (t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+  // the tangent is part of what a tensor without autograd data does not have
+  if (t.unsafeGetTensorImpl()->autograd_meta() && t._fw_grad(0).defined() &&
+      c10::AutogradState::get_tls_state().get_fw_grad_mode())
     value_error(std::string(name) +
                 ": has a tangent, and this operator has no forward gradient (use "
                 "torch.autograd.forward_ad.unpack_dual)");
@@ -301,11 +303,9 @@ PyObject* rms_norm(PyObject* const* a) {
   const void* r = nullptr;
   Tensor h;
   int64_t ldr = 0, ldh = 0;
-  const Memory mx = memory(x, rx);
-  Memory mr{}, mh{};
   auto apart = [&](const Memory& out, const char* name, bool in_place) {
-    check_apart(out, name, mx, "x", in_place);
-    if (r) check_apart(out, name, mr, "residual", in_place);
+    check_apart(out, name, memory(x, rx), "x", in_place);
+    if (r) check_apart(out, name, memory(THPVariable_Unpack(a[2]), "residual"), "residual", in_place);
     if (w) check_apart(out, name, memory(THPVariable_Unpack(a[1]), "weight"), "weight");
   };
   if (a[2] != Py_None) {
@@ -313,12 +313,11 @@ PyObject* rms_norm(PyObject* const* a) {
     if (res.sizes() != x.sizes())
       value_error("residual: expected shape " + text_of(x.sizes()) + ", got " +
                   text_of(res.sizes()));
-    mr = memory(res, "residual");
     ldr = rows(res, "residual").ld;
     r = res.const_data_ptr();
     h = output(a[7], x.sizes(), type, device, "residual_out");
     ldh = rows(h, "residual_out").ld;
-    if (a[7] != Py_None) apart(mh = memory(h, "residual_out"), "residual_out", true);
+    if (a[7] != Py_None) apart(memory(h, "residual_out"), "residual_out", true);
   } else if (a[7] != Py_None) {
     value_error("residual_out: given without a residual");
   }
@@ -327,7 +326,7 @@ PyObject* rms_norm(PyObject* const* a) {
   if (a[6] != Py_None) {
     const Memory my = memory(y, "out");
     apart(my, "out", !quant);
-    check_apart(my, "out", mh, "residual_out");
+    if (h.defined()) check_apart(my, "out", memory(h, "residual_out"), "residual_out");
   }
   Tensor s;
   int64_t lds = 0;
