@@ -582,8 +582,7 @@ int dense_w4(const DenseW4Args& a, int* status, cudaStream_t st) {
                 : nullptr;
   p.kblocks = a.w.kblocks();
   p.groups = a.w.groups();
-  p.rows = p.stage_blocks = p.recv_bytes = p.log_cluster = p.withhold = 0;
-  p.wait_ns = 0;
+  p.rows = p.stage_blocks = p.recv_bytes = p.log_cluster = 0;
   p.group_shift = -1;
   for (int l = 5; l < 31; ++l)
     if (a.w.group == 1 << l) p.group_shift = l;

@@ -68,9 +68,11 @@ struct Barriers {
   int abort_flag;
 };
 
+// expire_ns > 0: waits run out after it, and products never report their end
+// (b200_debug_w4_expire).
 template <int XT, int NC, int UNIT>
 __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
-    dense_w4_tc_kernel(const __grid_constant__ W4Params p, int* status) {
+    dense_w4_tc_kernel(const __grid_constant__ W4Params p, int* status, int64_t expire_ns) {
   using X = XRow<XT>;
   using Mma = typename X::Mma;
   using Raw = typename X::Raw;
@@ -104,6 +106,7 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
   float* recv = reinterpret_cast<float*>(cring + kExpanders * kCodeDepth * 1024);
   Barriers* bar = reinterpret_cast<Barriers*>(reinterpret_cast<char*>(recv) + p.recv_bytes);
   volatile int* abort_flag = &bar->abort_flag;
+  const uint64_t limit_ns = expire_ns > 0 ? (uint64_t)expire_ns : B200_WAIT_NS;
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&bar->full[i], (SB > 1 ? kExpanders : kExpanders / 2) + kStagers);
@@ -128,7 +131,7 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
   pdl_trigger();
   const uint32_t tmem = bar->tmem, tmem_sums = tmem + STAGES * SB * 32;
   auto wait = [&](uint64_t* b, int phase, int code) {
-    return mbar_wait_warp(b, phase & 1, status, code, abort_flag, p.wait_ns);
+    return mbar_wait_warp(b, phase & 1, status, code, abort_flag, limit_ns);
   };
   // the products of stage t's predecessor in the ring are done
   auto reusable = [&](int t) {
@@ -339,13 +342,13 @@ __global__ void __launch_bounds__(Stage<NC, UNIT>::kThreads, 1)
     }
   } else if (wid == kMmaWarp) {
     // ---- products
-    uint64_t* done = p.withhold ? bar->unheard : bar->done;
+    uint64_t* done = expire_ns > 0 ? bar->unheard : bar->done;
     for (int t = 0; lane == 0 && t < stages; ++t) {
       const int s = t % STAGES;
       if (!mbar_wait_long(&bar->full[s], (t / STAGES) & 1, status, kDevTimeoutFull, abort_flag,
-                          p.wait_ns) ||
+                          limit_ns) ||
           (t >= STAGES && !mbar_wait_long(&bar->taken[s], (t / STAGES - 1) & 1, status,
-                                          kDevTimeoutAccum, abort_flag, p.wait_ns)))
+                                          kDevTimeoutAccum, abort_flag, limit_ns)))
         break;
       tc_fence_after();
       const uint64_t bdesc = umma_desc_k<2, 1024>(smem_u32(xring + s * SB * NC * 128));
@@ -538,9 +541,6 @@ int launch(W4Params p, int* status, cudaStream_t st) {
   using S = Stage<NC, UNIT>;
   constexpr int PARTS = XRow<XT>::kParts;
   p.rows = NC / PARTS;
-  const int64_t expire = g_expire_ns.load(std::memory_order_relaxed);
-  p.wait_ns = expire > 0 ? (uint64_t)expire : B200_WAIT_NS;
-  p.withhold = expire > 0;
   const int64_t tiles = (p.a.w.N + kTileN - 1) / kTileN;
   const int64_t chunks = (p.a.M + p.rows - 1) / p.rows;
   if (chunks > 65535) return kErrTooLarge;
@@ -573,7 +573,8 @@ int launch(W4Params p, int* status, cudaStream_t st) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, status);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p, status,
+                                          g_expire_ns.load(std::memory_order_relaxed));
   count_launch();
   return launch_result(e != cudaSuccess ? e : cudaGetLastError());
 }

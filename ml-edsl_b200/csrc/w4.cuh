@@ -211,8 +211,6 @@ struct W4Params {
   int recv_bytes;    // of shared memory for other CTAs' sums
   int log_cluster;   // CTAs that share K
   int group_shift;   // log2 of the group, or -1
-  uint64_t wait_ns;  // limit of the tensor core kernel's waits
-  int withhold;      // its products never report their end (b200_debug_w4_expire)
   __device__ __forceinline__ unsigned group_of(int k) const {
     return group_shift >= 0 ? (unsigned)k >> group_shift : (unsigned)k / (unsigned)a.w.group;
   }
