@@ -52,35 +52,56 @@ def torch_commands():
     return compile_, link
 
 
-def needs_build():
-    if not (os.path.exists(LIB) and os.path.exists(TORCH_LIB)):
+def _stale(target):
+    """Whether a source is newer than `target`, or there is none."""
+    if not os.path.exists(target):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
+    t = os.path.getmtime(target)
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)]
     deps.append(os.path.join(HERE, "..", "include", "b200_edsl.h"))
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def needs_build():
+    return _stale(LIB) or _stale(TORCH_LIB)
+
+
 def build(force=False, verbose=False, extra=()):
-    if not force and not needs_build():
+    """The library needs the CUDA toolkit alone: it is built first and stays where
+    the torch module cannot be built (that is raised) or there is no torch (then
+    mlir_edsl.serving is not to be had)."""
+    lib, module = force or _stale(LIB), force or _stale(TORCH_LIB)
+    if not (lib or module):
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)
     cmd = [nvcc()] + NVCC_FLAGS + list(extra) + [os.path.join(CSRC, s) for s in SOURCES] + [
         "-o", LIB + ".tmp", "-lpthread"]
-    compile_, link = torch_commands()
-    if verbose:
-        print(" ".join(cmd), " ".join(compile_), " ".join(link), sep="\n")
-    beside = subprocess.Popen(compile_)
-    try:
-        subprocess.run(cmd, check=True)
+    if verbose and lib:
+        print(" ".join(cmd))
+    compiling = subprocess.Popen(cmd) if lib else None
+    failure, link = None, None
+    try:  # beside nvcc
+        if module:
+            compile_, link = torch_commands()
+            if verbose:
+                print(" ".join(compile_), " ".join(link), sep="\n")
+            subprocess.run(compile_, check=True)
+    except ImportError:
+        print("torch not found: mlir_edsl.serving is not built")
+    except (OSError, subprocess.CalledProcessError) as e:
+        failure = e
     finally:
-        rc = beside.wait()
+        rc = compiling.wait() if compiling else 0
     if rc:
-        raise subprocess.CalledProcessError(rc, compile_)
-    os.replace(LIB + ".tmp", LIB)
-    subprocess.run(link, check=True)
-    os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
-    os.remove(TORCH_LIB + ".o")
+        raise subprocess.CalledProcessError(rc, cmd)
+    if compiling:
+        os.replace(LIB + ".tmp", LIB)
+    if failure:
+        raise failure
+    if link:
+        subprocess.run(link, check=True)
+        os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
+        os.remove(TORCH_LIB + ".o")
     return LIB
 
 
