@@ -8,6 +8,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from importlib.metadata import PackageNotFoundError, version
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -15,6 +16,7 @@ LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libb200edsl.so")
 TORCH_SOURCE = os.path.join(CSRC, "torch_calls.cpp")
 TORCH_LIB = os.path.join(LIBDIR, "b200torch.so")
+TORCH_ABI = os.path.join(LIBDIR, "b200torch.abi")  # what it was compiled against
 SOURCES = ["gemm_tf32x3.cu", "gemm_i32.cu", "gemm_i32_tc.cu", "elementwise.cu", "runtime.cu", "noalloc.cu", "reduce.cu", "peer.cu",
            "rms_norm.cu", "dense_w4.cu", "dense_w4_tc.cu", "token_logprobs.cu", "serving.cu"]
 NVCC_FLAGS = [
@@ -62,15 +64,33 @@ def _stale(target):
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def torch_abi():
+    """What the torch module is compiled against, without importing torch."""
+    try:
+        return f"torch {version('torch')}, {sys.implementation.cache_tag}"
+    except PackageNotFoundError:
+        return "no torch"
+
+
+def _module_stale():
+    """Also where the module is another torch's or Python's, or of unknown ones."""
+    try:
+        with open(TORCH_ABI) as f:
+            built_for = f.read()
+    except FileNotFoundError:
+        built_for = None
+    return _stale(TORCH_LIB) or built_for != torch_abi()
+
+
 def needs_build():
-    return _stale(LIB) or _stale(TORCH_LIB)
+    return _stale(LIB) or _module_stale()
 
 
 def build(force=False, verbose=False, extra=()):
     """The library needs the CUDA toolkit alone: it is built first and stays where
     the torch module cannot be built (that is raised) or there is no torch (then
     mlir_edsl.serving is not to be had)."""
-    lib, module = force or _stale(LIB), force or _stale(TORCH_LIB)
+    lib, module = force or _stale(LIB), force or _module_stale()
     if not (lib or module):
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)
@@ -102,6 +122,8 @@ def build(force=False, verbose=False, extra=()):
         subprocess.run(link, check=True)
         os.replace(TORCH_LIB + ".tmp", TORCH_LIB)
         os.remove(TORCH_LIB + ".o")
+        with open(TORCH_ABI, "w") as f:
+            f.write(torch_abi())
     return LIB
 
 

@@ -4,6 +4,7 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
 import build
 
@@ -32,6 +33,7 @@ def fake(tmp_path, monkeypatch):
     monkeypatch.setattr(build, "LIBDIR", str(tmp_path / "lib"))
     monkeypatch.setattr(build, "LIB", str(tmp_path / "lib" / "libb200edsl.so"))
     monkeypatch.setattr(build, "TORCH_LIB", str(tmp_path / "lib" / "b200torch.so"))
+    monkeypatch.setattr(build, "TORCH_ABI", str(tmp_path / "lib" / "b200torch.abi"))
     monkeypatch.setattr(build, "nvcc", lambda: f.tool("nvcc"))
     monkeypatch.setattr(build, "torch_commands", lambda: (
         [f.tool("g++"), "-o", build.TORCH_LIB + ".o"], [f.tool("ld"), "-o", build.TORCH_LIB + ".tmp"]))
@@ -42,7 +44,7 @@ def test_both_are_built(fake):
     assert build.needs_build()
     build.build()
     assert os.path.exists(build.LIB) and os.path.exists(build.TORCH_LIB)
-    assert sorted(os.listdir(build.LIBDIR)) == ["b200torch.so", "libb200edsl.so"]
+    assert sorted(os.listdir(build.LIBDIR)) == ["b200torch.abi", "b200torch.so", "libb200edsl.so"]
     calls = fake.calls()
     assert sorted(calls) == ["g++", "ld", "nvcc"] and not build.needs_build()
     build.build()
@@ -70,3 +72,15 @@ def test_a_library_that_fails_is_raised(fake):
     with pytest.raises(subprocess.CalledProcessError):
         build.build()
     assert not os.path.exists(build.LIB) and not os.path.exists(build.TORCH_LIB)
+
+
+def test_the_module_is_built_again_for_another_torch(fake, monkeypatch):
+    build.build()
+    now = build.torch_abi()
+    assert torch.__version__ in now
+    monkeypatch.setattr(build, "torch_abi", lambda: now + ".1")
+    assert build.needs_build()
+    build.build()
+    assert sorted(fake.calls()) == ["g++", "g++", "ld", "ld", "nvcc"] and not build.needs_build()
+    os.remove(build.TORCH_ABI)  # built by who knows what
+    assert build.needs_build()
