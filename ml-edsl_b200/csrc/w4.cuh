@@ -12,7 +12,6 @@ namespace b200 {
 
 constexpr int kBlockK = 64;     // k of one packed block
 constexpr int kStripN = 64;     // columns of one strip
-constexpr int kMaxCluster = 8;  // CTAs that share K
 
 // Place of column n (within its strip) among a group's 64 scales or zeros:
 // lane group g = n % 8 reads its eight values together.
