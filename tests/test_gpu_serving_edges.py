@@ -279,3 +279,136 @@ def test_rms_norm_scales_of_rows_without_columns(cuda):
     q, s = serving.rms_norm(x, torch.empty(0, device=cuda), quant="e4m3", group=32)
     synced()
     assert q.shape == (5, 0) and s.shape == (5, 0)
+
+
+# ----------------------------------------------- forms of calls not tested elsewhere
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, E4M3])
+@pytest.mark.parametrize("M", [3, 20, 100])
+def test_dense_w4_without_columns_of_x(cuda, dtype, M):
+    none = serving.pack_w4(torch.empty(0, 130, dtype=torch.uint8, device=cuda),
+                           torch.empty(0, 130, device=cuda))
+    bias = rand(cuda, 2, 130)
+    y = serving.dense_w4(torch.empty(M, 0, device=cuda, dtype=dtype), none, bias, act=1,
+                         out_dtype=F32)
+    synced()
+    assert torch.equal(y, bias.clamp(min=0).expand(M, 130))
+
+
+@pytest.mark.parametrize("M", [1, 2, 4])
+def test_dense_w4_keeps_all_bits_of_f32_rows(cuda, M):
+    """One product in each row, on both kernels: up to 2 rows of f32 and more."""
+    K = 256
+    codes = torch.full((K, 64), 8, dtype=torch.uint8, device=cuda)
+    codes[3], codes[200] = 9, 15
+    w = serving.pack_w4(codes, torch.ones(2, 64, device=cuda))
+    for at, value in ((3, 1 + 2.0 ** -23), (3, -3.4e38), (200, 1.7654321), (200, 2.0 ** -100),
+                      (3, 1.9999999), (3, -1.0000001e-20)):
+        x = torch.zeros(M, K, device=cuda)
+        x[M - 1, at] = value
+        y = serving.dense_w4(x, w)
+        synced()
+        want = (x[:, at].double() * (1 if at == 3 else 7)).float()
+        assert torch.equal(y, want[:, None].expand(M, 64))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 2, 8, 9, 33, 100])
+def test_dense_w4_sums_by_unit(cuda, dtype, group, M):
+    """Errors against the additions that the kernels make: within a unit of K
+    (32 in groups of 32; 128 in groups of 128 on the tensor core; otherwise 64)
+    one k16 step after another, two truncations of 2^-22 of the sum of absolute
+    products each; then one f32 addition a unit and 16 for parts, warps, CTAs."""
+    K, N = 4096, 192
+    g = torch.Generator(device=cuda).manual_seed(M)
+    codes = torch.randint(0, 16, (K, N), device=cuda, generator=g, dtype=torch.uint8)
+    scales = (torch.rand(K // group, N, device=cuda, generator=g) + 0.5).to(dtype)
+    W = (codes.double() - 8) * scales.double()[torch.arange(K, device=cuda) // group]
+    x = rand(cuda, M, M, K).to(dtype)
+    y = serving.dense_w4(x, serving.pack_w4(codes, scales, group=group), out_dtype=F32)
+    synced()
+    columns = M * (3 if dtype == F32 else 1)
+    unit = 32 if group == 32 else 128 if group == 128 and columns > 8 else 64
+    room = unit / 16 * 2 * 2.0 ** -22 + (K // unit + 16) * 2.0 ** -24 + 2.0 ** -24
+    size = x.double().abs() @ W.abs()
+    assert ((y.double() - x.double() @ W).abs() <= room * size).all()
+
+
+@pytest.mark.parametrize("x_group", [32, 64, 128])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_dense_w4_many_scaled_rows(cuda, x_group, group):
+    M, K, N = 100, 1000, 192
+    g = torch.Generator(device=cuda).manual_seed(7)
+    codes = torch.randint(0, 16, (K, N), device=cuda, generator=g, dtype=torch.uint8)
+    parts = -(-K // group)
+    scales = torch.rand(parts, N, device=cuda, generator=g) + 0.5
+    W = (codes.double() - 8) * scales.double()[torch.arange(K, device=cuda) // group]
+    x = rand(cuda, M, M, K).to(E4M3)
+    s = rand(cuda, 9, M, -(-K // x_group)).abs() + 0.1
+    y = serving.dense_w4(x, serving.pack_w4(codes, scales, group=group), x_scales=s,
+                         x_group=x_group, out_dtype=F32)
+    synced()
+    xd = x.double() * s.double().repeat_interleave(x_group, 1)[:, :K]
+    size = xd.abs() @ W.abs()
+    # as above with the smallest unit's additions and the longest unit's steps,
+    # and one rounding more for the second scale
+    room = 16 * 2.0 ** -22 + (K / 32 + 16 + 2) * 2.0 ** -24
+    assert ((y.double() - xd @ W).abs() <= room * size).all()
+
+
+def test_token_logprobs_of_many_rows_in_one_thread(cuda):
+    """Rows of one CTA each whose most probable tokens all lie in the 16-byte
+    chunks of one of its 256 threads."""
+    T, V = 300, 256 * 8 * 40
+    logits = rand(cuda, 1, T, V).bfloat16()
+    at = torch.arange(40, device=cuda) * 256 * 8 + 24
+    logits[:, at] = (20 + torch.arange(40, device=cuda).float()).bfloat16()
+    logits[:, at + 1] = 21
+    out = serving.token_logprobs(logits, top=32)
+    synced()
+    for i in range(0, T, 50):
+        x = logits[i:i + 50].double()
+        order = torch.sort(x, dim=1, descending=True, stable=True)
+        assert torch.equal(out.top_tokens[i:i + 50].long(), order.indices[:, :32])
+        want = order.values[:, :32] - torch.logsumexp(x, 1, keepdim=True)
+        # e^t to some steps of 2^-23, at most 320 of them in a thread's sum, 16 joins
+        room = (320 / 2 + 92) * 2.0 ** -23 + 2.0 ** -22 * (want.abs() + 64)
+        assert ((out.top_logprobs[i:i + 50].double() - want).abs() <= room).all()
+
+
+def test_calls_from_several_threads(cuda):
+    """Threads on streams of their own get what one thread gets."""
+    import threading
+    w = serving.quantize_w4(rand(cuda, 1, 512, 3001), group=64)
+    norm = rand(cuda, 2, 512)
+    rows = [rand(cuda, 3 + i, 1 + 7 * i, 512).bfloat16() for i in range(4)]
+
+    def served(x):
+        q, s, h = serving.rms_norm(x, norm, residual=x, quant="e4m3", group=128)
+        logits = serving.dense_w4(q, w, x_scales=s, x_group=128, out_dtype=F32)
+        return (h, logits) + serving.token_logprobs(logits, top=7)[1:]
+
+    want = [served(x) for x in rows]
+    synced()
+    got, wrong = [None] * 4, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()) as _:
+                for _ in range(50):
+                    got[i] = served(rows[i])
+                    if not all(torch.equal(a, b) for a, b in zip(got[i], want[i])):
+                        wrong.append(i)
+                with pytest.raises(ValueError):
+                    serving.rms_norm(rows[i], group=i + 1)
+        except BaseException as e:  # a thread's failure is the test's
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    synced()
+    assert not wrong, wrong
