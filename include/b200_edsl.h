@@ -379,9 +379,9 @@ int b200_w4_dequantize(const void* packed, int s_dtype, int has_zeros, int64_t K
  * bf16 or f16. An e4m3 X may have x_scales: one for each row (x_group 0,
  * x_scales[m * ld_x_scales]) or for each x_group (32, 64 or 128) columns, as
  * b200_rms_norm writes them. Products are exact and sums run in f32, with an f32
- * X's every bit; no sum leaves f32's range before its scale is applied (for an X
- * of f32 or bf16 sums are kept divided by 4096, so results below 2^-114 have the
- * bits that f32 has below 2^-126). Y is rounded once. Up to 8 rows (f32: 2) run
+ * X's every bit down to 2^-133; no sum leaves f32's range before its scale is
+ * applied (for an X of f32 or bf16 sums are kept divided by 4096, so what they
+ * have below 2^-137 is lost). Y is rounded once. Up to 8 rows (f32: 2) run
  * on mma.sync, more on tcgen05; the weights are read once for each 128 rows (64
  * with groups of 32; f32: a third of that), so several hundred rows are better
  * served by b200_w4_dequantize and b200_dense_f32. The first call on a device

@@ -11,10 +11,10 @@
 // so the products are taken by mma.sync m16n8k16 with the weights as the
 // 16-row operand (16 columns of W) and the rows of X as its 8 columns:
 // x of bf16 as it is; f16 and e4m3 as f16 (exact); f32 as the sum of three
-// bf16 parts of 8 bits each (exact), in three columns that are added at the
-// end. bf16 weights are (q - z) / 4096 until the end, so that no sum before the
-// scale leaves f32's range; what that costs lies below 2^-114. No product is
-// rounded; sums run in f32, in the tensor core within a
+// bf16 parts of 8 bits each (exact down to bf16's smallest value, 2^-133), in three
+// columns that are added at the end. bf16 weights are (q - z) / 4096 until the end,
+// so that no sum before the scale leaves f32's range; what that costs lies below
+// 2^-137. No product is rounded; sums run in f32, in the tensor core within a
 // group (or a 64-long part of one), then with ordinary adds after the scale
 // is applied in f32. For up to 8 operand columns the codes go from HBM to
 // registers and into the product within one warp; more columns are

@@ -412,3 +412,66 @@ def test_calls_from_several_threads(cuda):
         t.join()
     synced()
     assert not wrong, wrong
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M", [2, 20])
+def test_dense_w4_of_tiny_rows(cuda, dtype, M):
+    """Sums are kept divided by 4096, so bits below 2^-149 * 4096 = 2^-137 are lost:
+    no more than two such steps for each of K products, times the scale. And the
+    bf16 parts of an f32 x have no bits below bf16's smallest value, 2^-133: less
+    than that is lost of each x."""
+    K, N = 128, 70
+    g = torch.Generator(device=cuda).manual_seed(M)
+    codes = torch.randint(0, 16, (K, N), device=cuda, generator=g, dtype=torch.uint8)
+    scales = torch.rand(2, N, device=cuda, generator=g) + 0.5
+    W = (codes.double() - 8) * scales.double()[torch.arange(K, device=cuda) // 64]
+    x = (rand(cuda, M, M, K) * 2.0 ** -118).to(dtype)
+    y = serving.dense_w4(x, serving.pack_w4(codes, scales, group=64), out_dtype=F32)
+    synced()
+    size = x.double().abs() @ W.abs()
+    room = 2 * K * 1.5 * 2.0 ** -137 + 2.0 ** -18 * size
+    if dtype == F32:
+        room = room + 2.0 ** -133 * W.abs().sum(0)
+    assert ((y.double() - x.double() @ W).abs() <= room).all()
+
+
+def test_frontend_operators_alone_and_4_bits_on_the_left(cuda):
+    """Functions of one step; weights in 4 bits count where they are the right
+    operand of a product, and as f32 everywhere else."""
+    import numpy as np
+    from mlir_edsl import (Tensor, f32, i32, ml_function, register_weights, release_weights,
+                           rms_norm, token_logprobs)
+
+    @ml_function(target="b200")
+    def norm(X: Tensor[f32, 5, 64]) -> Tensor[f32, 5, 64]:
+        return rms_norm(X)
+
+    @ml_function(target="b200")
+    def score(X: Tensor[f32, 5, 64], t: Tensor[i32, 5]) -> Tensor[f32, 5]:
+        return token_logprobs(X, t)
+
+    @ml_function(target="b200")
+    def twice(A: Tensor[f32, 64, 64], W: Tensor[f32, 64, 64]) -> Tensor[f32, 64, 64]:
+        return (A @ W) @ W
+
+    rng = np.random.default_rng(1)
+    X, W = (rng.standard_normal((n, 64)).astype(np.float32) for n in (5, 64))
+    x = torch.from_numpy(X).double()
+    want = x / torch.sqrt((x * x).mean(1, keepdim=True) + 1e-6)
+    assert (np.abs(norm(X) - want.numpy()) <= NORM_F32 * np.abs(want.numpy()) + 2.0 ** -149).all()
+    got = score(X, np.array([3, 0, -1, 63, 64], np.int32))
+    logs = torch.log_softmax(x, 1)
+    assert np.abs(got[[0, 1, 3]] - [logs[0, 3], logs[1, 0], logs[3, 63]]).max() <= 2.0 ** -18
+    assert got[2] == 0 and np.isnan(got[4])
+    register_weights(W, bits=4, group=64)
+    try:
+        left = twice(W, W)
+    finally:
+        release_weights(W)
+    D = serving.quantize_w4(torch.from_numpy(W).to(cuda), group=64).dequantize().cpu().double()
+    w = torch.from_numpy(W).double()
+    inner = w @ D
+    # 2^-18 of the sum of absolute products in each layer, carried through the second
+    room = 2.0 ** -18 * (w.abs() @ D.abs() @ D.abs() + inner.abs() @ D.abs())
+    assert (np.abs(left - (inner @ D).numpy()) <= room.numpy()).all()
