@@ -213,11 +213,13 @@ __global__ void w4_dequantize_kernel(const uint32_t* __restrict__ codes, const c
 // part of K are staged once, or stage_blocks of K at a time where that takes
 // more than kXBytes.
 //
-// Bound by issue, not yet by HBM: about 340 instructions for a block and strip
+// Bound by instructions, not yet by HBM: about 340 of a warp for a block and strip
 // (4096 weights: 176 to expand them, 16 products, 16 sums, the rest copies and
-// addresses) keep the schedulers at 45%. 1x4096x4096 bf16 5.3 us (floor 1.3),
-// 1x8192x16384 22.5 us or 3.1 TB/s (floor 10.6); with four warps a CTA and four
-// CTAs an SM 5.7 and 26.5 us, with six blocks ahead 32.5 us for the latter.
+// addresses), 2.6 of a thread for a weight; the schedulers issue in 51% of cycles
+// (1x8192x16384). 1x4096x4096 bf16 5.3 us (floor 1.3), 1x8192x16384 22.2 us or
+// 3.1 TB/s (floor 10.6); with four warps a CTA and four CTAs an SM 5.7 and 26.5 us,
+// with six blocks ahead 32.5 us for the latter. 1x4096x11008 f32, whose variant
+// spills 48 bytes, lost by it: 13.8 us with four warps, 14.5 with eight.
 constexpr int kFewWarps = 8;
 constexpr int kFewColumns = 8;  // operand columns of a CTA
 constexpr int kDepth = 4;

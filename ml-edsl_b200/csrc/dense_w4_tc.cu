@@ -18,7 +18,9 @@
 // few rows. Measured on B200, a product of up to 64 columns takes 47 cycles to
 // issue, a commit 190 and each meeting of two roles about as long, so they
 // meet once for a stage of up to four blocks of K, with one commit for its
-// operands and its sums. Waits between the roles are bounded; one that runs out
+// operands and its sums. 17 or 21 warps leave 96 or 80 registers for every role:
+// variants of 128 columns and most for e4m3 spill. 64x8192x8192 f16 23.1 us (floor
+// 5.6), 5.7 thread instructions a weight in 57% of issue slots. Waits between the roles are bounded; one that runs out
 // ends all of them, makes what the cluster stores NaN and is reported by
 // b200_stream_sync. (The allocation of TMEM and the cluster's barriers wait for
 // other CTAs to run or to end, which these bounds see to.)

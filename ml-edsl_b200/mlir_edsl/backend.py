@@ -101,7 +101,8 @@ def register_weights(W: np.ndarray, version: int = 0, *, bits: int = 32,
 
     bits=4 keeps W in 4 bits instead, with a scale for each `group` (32 or a
     multiple of 64) rows of each column (b200_weights_register_w4): functions
-    that multiply by W then do so by its 4-bit values."""
+    that have W as the right operand of a product then use its 4-bit values
+    there (its f32 values everywhere else), on the current device alone."""
     if not isinstance(W, np.ndarray) or W.dtype != np.float32 or W.ndim != 2:
         raise TypeError("register_weights takes a 2-D float32 ndarray")
     if not W.flags["C_CONTIGUOUS"]:

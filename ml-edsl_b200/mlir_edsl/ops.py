@@ -29,7 +29,8 @@ def leaky_relu(arr: Value, alpha: float = 0.01) -> LinalgActivation:
 
 def rms_norm(arr: Value, weight: Value = None, residual: Value = None, eps: float = 1e-6):
     """h / sqrt(mean(h^2) + eps) * weight over the rows of a 2-D f32 tensor,
-    h = arr (+ residual). No counterpart in the reference."""
+    h = arr (+ residual); h itself is not returned. No counterpart in the
+    reference."""
     from .ast import RmsNorm
     return RmsNorm(arr, weight, residual, eps)
 
