@@ -475,3 +475,75 @@ def test_frontend_operators_alone_and_4_bits_on_the_left(cuda):
     # 2^-18 of the sum of absolute products in each layer, carried through the second
     room = 2.0 ** -18 * (w.abs() @ D.abs() @ D.abs() + inner.abs() @ D.abs())
     assert (np.abs(left - (inner @ D).numpy()) <= room.numpy()).all()
+
+
+# ------------------------------------------------- offsets past 2^31 elements
+
+@pytest.fixture
+def room(cuda):
+    """Fresh memory before and after a test of some GB."""
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("M,N,quant", [(540000, 4096, True), (540000, 4091, True),
+                                       (70000, 32768, False)])
+def test_rms_norm_far_rows(cuda, room, M, N, quant):
+    x = torch.zeros(M, N, dtype=BF16, device=cuda)
+    last = [0, M // 2, M - 2, M - 1]
+    x[last] = rand(cuda, 1, 4, N).bfloat16()
+    w = (rand(cuda, 2, N) * 0.1 + 1).bfloat16()
+    out = serving.rms_norm(x, w, quant="e4m3", group=128) if quant else serving.rms_norm(x, w)
+    synced()
+    want = norm_formula(x[last], 1e-6) * w.double()
+    if not quant:
+        room = half_step(want, BF16) + NORM_F32 * want.abs()
+        assert ((out[last].double() - want).abs() <= room).all() and (out[M - 3] == 0).all()
+        return
+    codes, scales = out
+    assert (scales[M - 3] == 1).all() and (scales[M // 2 + 1] == 1).all()
+    assert (codes[M - 3].float() == 0).all()
+    per = scales[last].double().repeat_interleave(128, 1)[:, :N]
+    for i, g0 in enumerate(range(0, N, 128)):
+        most = want[:, g0:g0 + 128].abs().amax(1) / 448
+        assert ((scales[last, i].double() - most).abs() <= 2 * NORM_F32 * most).all()
+    # half a step of e4m3 of the value, or near 0 of its smallest one
+    step = torch.maximum(want.abs() * 2.0 ** -4, per * 2.0 ** -10)
+    value = codes[last].double() * per
+    assert ((value - want).abs() <= step * (1 + 2.0 ** -10) + 4 * NORM_F32 * want.abs()).all()
+
+
+def test_token_logprobs_far_rows(cuda, room):
+    T, V = 20000, 131072
+    logits = torch.zeros(T, V, dtype=F16, device=cuda)
+    last = [0, T // 2, T - 1]
+    logits[last] = (rand(cuda, 1, 3, V) * 3).half()
+    tokens = torch.arange(T, dtype=torch.int32, device=cuda)
+    out = serving.token_logprobs(logits, tokens, top=5)
+    synced()
+    for i, row in enumerate(last):
+        x = logits[row].double()
+        order = torch.sort(x, descending=True, stable=True)
+        lse = torch.logsumexp(x, 0)
+        assert torch.equal(out.top_tokens[row].long(), order.indices[:5])
+        # as for rows of one thread's tokens, with 512 logits a thread
+        assert ((out.top_logprobs[row].double() - (order.values[:5] - lse)).abs() <= 2.0 ** -13).all()
+        assert abs(out.logprobs[row].double() - (x[row] - lse)) <= 2.0 ** -13
+    assert (out.top_tokens[T - 2] == torch.arange(5, device=cuda)).all()
+
+
+@pytest.mark.parametrize("M", [5, 17])
+def test_dense_w4_far_rows(cuda, room, M):
+    """Rows of X and of Y that lie 2^32 bytes apart and more."""
+    K, N, far = 256, 130, (1 << 32) // (M - 1) + 64
+    w = serving.quantize_w4(rand(cuda, 1, K, N), group=64)
+    x = torch.empty((M - 1) * far + K, dtype=BF16, device=cuda).as_strided((M, K), (far, 1))
+    y = torch.empty((M - 1) * far + N, dtype=BF16, device=cuda).as_strided((M, N), (far, 1))
+    x.copy_(rand(cuda, 2, M, K))
+    want = serving.dense_w4(x.contiguous(), w)
+    serving.dense_w4(x, w, out=y)
+    synced()
+    assert torch.equal(y, want)
