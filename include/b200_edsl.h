@@ -343,13 +343,14 @@ int b200_host_free(void* ptr);
  *   h = X + R;  y = h / sqrt(mean(h^2) + eps) * w
  * X, R (or NULL) and H (or NULL: not stored) are of type `dtype`; w[N] (or
  * NULL: 1) is of that type or f32. H, and a Y of X's type, may be X or R itself
- * (same address and pitch; not both the same one). y is computed in f32 from the f32 sum and rounded once into Y:
- * of X's type (y_dtype == dtype, scales NULL), or e4m3 codes
- * (y_dtype B200_E4M3) with scales: the value is code * scale, and
+ * (same address and pitch; not both the same one). y is computed in f32 from the
+ * f32 sum and rounded once into Y: of X's type (y_dtype == dtype, scales NULL),
+ * or e4m3 codes (y_dtype B200_E4M3) with scales: the value is code * scale, and
  * scale = max|y| / 448 over the row (group 0: scales[m * ld_scales]) or over
  * each `group` (32, 64 or 128) columns (scales[m * ld_scales + n / group];
- * the last group may be shorter). Where all of y is zero the scale is 1. A
- * row of X that holds an infinity or NaN gives what the formula gives. */
+ * the last group may be shorter). Where all of y is zero, or there is none (N 0,
+ * group 0), the scale is 1. A row of X that holds an infinity or NaN gives what
+ * the formula gives. */
 int b200_rms_norm(const void* X, int64_t ldx, const void* R, int64_t ldr, int dtype, const void* w,
                   int w_dtype, float eps, void* H, int64_t ldh, void* Y, int64_t ldy, int y_dtype,
                   float* scales, int64_t ld_scales, int group, int64_t M, int64_t N, void* stream);
